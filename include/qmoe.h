@@ -290,6 +290,75 @@ int qmoe_router_logits(const float* x, int tokens, int d_model, const float* rou
  * streaming-read ceiling of the device for a launch of that size. */
 int qmoe_read_probe(const void* buffer, size_t bytes, uint32_t match, uint32_t* sink, void* stream);
 
+/* ---- 8-bit integer weights and activations ----------------------------------------------------
+ * Codes with a scale for each output channel (weights) and for each token (activations); no
+ * counterpart in the reference, whose packed products keep activations in floating point.
+ *     q[t, k] = rint(x[t, k] / s[t]),  s[t] = fl32(max_k |x[t, k]| / 127)   halves to even, |q| <= 127
+ *     y[t, n] = (sum_k q[t, k] w[n, k]) * s[t] * c[n]                       int32 sum, exact
+ * s[t] == 0 makes all codes 0; a row with a NaN or an infinity gets s[t] = NaN and codes of 0, so its
+ * products are NaN.  Weights are any int8 codes with fp32 scales, laid out once as tiles of 16
+ * channels x 64 columns (qmoe_int8_tiles), zero-padded.  K <= 131071, where the int32 sum cannot
+ * overflow.  These functions were added without a change of QMOE_ABI_VERSION: nothing that was there
+ * changed. */
+enum { QMOE_DT_INT8 = 3 };   /* x_dtype of the products: codes given by the caller, with x_scales */
+
+/* Bytes of the tiles of an [n, k] matrix: n rounded up to 16, times k rounded up to 64. */
+size_t qmoe_int8_matrix_bytes(int n, int k);
+
+/* codes[rows, k] int8 and scales[rows] fp32 of contiguous x [rows, k] (fp32 / fp16 / bf16). */
+int qmoe_int8_quantize(const void* x, int x_dtype, int64_t rows, int k, void* codes, float* scales, void* stream);
+
+/* `matrices` row-major code matrices [n, k], one behind the other, to tiles (16-byte aligned), one
+ * matrix every qmoe_int8_matrix_bytes(n, k) bytes. */
+int qmoe_int8_tiles(const void* codes, int64_t matrices, int n, int k, void* tiles, void* stream);
+
+/* Bytes of workspace of the two products below (not needed for codes of k % 64 == 0 at a 16-byte
+ * aligned address). */
+size_t qmoe_int8_workspace_bytes(int n, int k, int tokens);
+
+/* y[tokens, n] as above, rounded once to y_dtype.  x: contiguous [tokens, k] in fp32 / fp16 / bf16,
+ * quantised on the way (x_scales ignored), or QMOE_DT_INT8 with x_scales[tokens]. */
+int qmoe_int8_linear(const void* tiles, const float* channel_scales, int n, int k, const void* x, int x_dtype,
+                     const float* x_scales, int tokens, void* y, int y_dtype, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* h[tokens, f] = silu(x @ G^T) * (x @ U^T) on the same terms; gate and up share [f, k]. */
+int qmoe_int8_swiglu(const void* gate, const float* gate_scales, const void* up, const float* up_scales, int f, int k,
+                     const void* x, int x_dtype, const float* x_scales, int tokens, void* h, int h_dtype,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* One MoE step on such weights.  Host struct; fields as in qmoe_moe_args, matrices as tiles: gate / up
+ * n_experts x [d_ff, d_model], down n_experts x [d_model, d_ff], each with fp32 channel scales
+ * [n_experts, rows]; the shared expert (all NULL and d_ff_shared = 0: none) likewise.  Every expert's
+ * hidden activation is rounded to fp32 and quantised per (token, expert) before its down projection. */
+typedef struct qmoe_int8_moe_args {
+    const void* hidden;
+    int hidden_dtype;
+    int tokens;
+    int top_k;
+    const float* logits;
+    float floor_value;
+    int renormalize;
+    const float* in_weights;
+    const int64_t* in_ids;
+    const void *gate, *up, *down;
+    const float *gate_scales, *up_scales, *down_scales;
+    int n_experts, d_model, d_ff;
+    const void *shared_gate_w, *shared_up_w, *shared_down_w;
+    const float *shared_gate_scales, *shared_up_scales, *shared_down_scales;
+    int d_ff_shared;
+    const float* shared_gate;
+    void* out;
+    int out_dtype;
+    float* out_weights;
+    int64_t* out_ids;
+    const float* residual;
+    int* status_out;
+} qmoe_int8_moe_args;
+
+size_t qmoe_int8_moe_workspace_bytes(int tokens, int top_k, int n_experts, int d_model, int d_ff, int d_ff_shared);
+int qmoe_int8_moe_forward(const qmoe_int8_moe_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- host twins -----------------------------------------------------------------------------
  * The same operators over HOST pointers, computed on the CPU by one thread of scalar C++ (no
  * stream, nothing touches the GPU).  They serve callers that hold NumPy activations and

@@ -43,6 +43,17 @@ class MoeArgs(ctypes.Structure):
                 ("out", _P), ("out_dtype", _I), ("out_weights", _P), ("out_ids", _P), ("residual", _P), ("status_out", _P)]
 
 
+class Int8MoeArgs(ctypes.Structure):
+    _fields_ = [("hidden", _P), ("hidden_dtype", _I), ("tokens", _I), ("top_k", _I),
+                ("logits", _P), ("floor_value", _F), ("renormalize", _I), ("in_weights", _P), ("in_ids", _P),
+                ("gate", _P), ("up", _P), ("down", _P), ("gate_scales", _P), ("up_scales", _P), ("down_scales", _P),
+                ("n_experts", _I), ("d_model", _I), ("d_ff", _I),
+                ("shared_gate_w", _P), ("shared_up_w", _P), ("shared_down_w", _P),
+                ("shared_gate_scales", _P), ("shared_up_scales", _P), ("shared_down_scales", _P),
+                ("d_ff_shared", _I), ("shared_gate", _P),
+                ("out", _P), ("out_dtype", _I), ("out_weights", _P), ("out_ids", _P), ("residual", _P), ("status_out", _P)]
+
+
 ABI_VERSION = 5   # QMOE_ABI_VERSION of include/qmoe.h this binding was written against
 
 _SIGNATURES = {
@@ -66,6 +77,14 @@ _SIGNATURES = {
     "qmoe_router_logits": ([_P, _I, _I, _P, _P, _I, _P, _P], _I),
     "qmoe_routing_plan": ([_P, _P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P], _I),
     "qmoe_read_probe": ([_P, _SZ, ctypes.c_uint32, _P, _P], _I),
+    "qmoe_int8_matrix_bytes": ([_I, _I], _SZ),
+    "qmoe_int8_quantize": ([_P, _I, _I64, _I, _P, _P, _P], _I),
+    "qmoe_int8_tiles": ([_P, _I64, _I, _I, _P, _P], _I),
+    "qmoe_int8_workspace_bytes": ([_I, _I, _I], _SZ),
+    "qmoe_int8_linear": ([_P, _P, _I, _I, _P, _I, _P, _I, _P, _I, _P, _SZ, _P], _I),
+    "qmoe_int8_swiglu": ([_P, _P, _P, _P, _I, _I, _P, _I, _P, _I, _P, _I, _P, _SZ, _P], _I),
+    "qmoe_int8_moe_workspace_bytes": ([_I, _I, _I, _I, _I, _I], _SZ),
+    "qmoe_int8_moe_forward": ([ctypes.POINTER(Int8MoeArgs), _P, _SZ, _P], _I),
     "qmoe_dequantize_cpu": ([_P, _I, _I64, _I64, _P], _I),
     "qmoe_linear_cpu": ([_P, _I, _I, _I, _P, _I, _P], _I),
     "qmoe_swiglu_cpu": ([_P, _I, _P, _I, _I, _I, _P, _I, _P], _I),

@@ -1,0 +1,105 @@
+// 8-bit integer operators: codes with a scale for each token (activations) and for each output
+// channel (weights).
+//
+//   q[t, k] = rint(x[t, k] / s[t]),  s[t] = fl32(max_k |x[t, k]| / 127)      (halves to even, |q| <= 127)
+//   y[t, n] = (sum_k q[t, k] w[n, k]) * s[t] * c[n]                            (int32 sum: exact)
+//
+// Weight layout ("tiles"): [N/16][K/64][lane][16] bytes, lane l of a 1 KB tile holding columns
+// 16 (l / 16) .. + 15 of row l % 16 -- the A operand of v_mfma_i32_16x16x64_i8 as a wave reads it,
+// 1 KB of consecutive memory an instruction.  Rows are padded to 16 and columns to 64 with zero
+// codes, so what an activation row holds behind its K columns never counts.  Activation codes are
+// row-major with a row step that is a multiple of 16 bytes and at least K rounded up to 64: lane l
+// reads the B operand as the 16 bytes at column 16 (l / 16) of token l % 16.  D[i] of lane l is the
+// sum of weight row 4 (l / 16) + i and token l % 16: four neighbouring outputs of one token.
+#pragma once
+#include "qmoe_common.hpp"
+
+namespace qmoe {
+
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+
+static constexpr int INT8_MAX_K = 131071;     // 128 * 128 * K stays inside int32
+static constexpr int QMOE_DT_I8 = QMOE_DT_INT8;
+
+__host__ __device__ inline int64_t int8_rows16(int64_t n) { return (n + 15) / 16 * 16; }
+__host__ __device__ inline int64_t int8_cols64(int64_t k) { return (k + 63) / 64 * 64; }
+inline int64_t int8_matrix_bytes(int64_t n, int64_t k) { return int8_rows16(n) * int8_cols64(k); }
+
+__device__ __forceinline__ i32x4_t mfma_i8(i32x4_t a, i32x4_t b, i32x4_t c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ i32x4_t ldg_i32x4(const void* p) { return *(const QMOE_GLOBAL i32x4_t*)p; }
+
+// The scale of a row and what its codes are made with.  `top` is the largest |x| of the row as bits
+// (NaN and infinity compare above every finite value).  A row that is not finite gets the scale NaN
+// and codes of zero, so that every product of that row is NaN instead of a plausible number.
+struct RowScale {
+    float s;
+    double inv;      // 1 / s, or 0 where all codes are 0
+    __device__ __forceinline__ explicit RowScale(uint32_t top) {
+        const bool finite = top < 0x7F800000u;
+        s = finite ? __fdiv_rn(__uint_as_float(top), 127.0f) : __uint_as_float(0x7FC00000u);
+        inv = finite && s > 0.0f ? 1.0 / (double)s : 0.0;
+    }
+};
+
+// rint(x / s), halves to even, as if the quotient were exact.  x * inv is off by less than 2^-44; a
+// quotient of two fp32 values that is not exactly n + 1/2 is at least 2^-25 away from it (x / s - (2n + 1) / 2
+// = (2x - (2n + 1) s) / 2s, and the numerator is a multiple of the smaller of the two last places).
+// Rounding to multiples of 2^-40 first therefore puts every tie on the tie and moves nothing across it.
+// (an infinite x of a row without a scale would make a NaN here: the caller's row has inv = 0 and the
+// comparison below sends it to 0)
+__device__ __forceinline__ int int8_code(float x, double inv) {
+    const double snap = 6144.0;      // 1.5 * 2^12: the last place of a sum is 2^-40
+    const double t = ((double)x * inv + snap) - snap;
+    const double r = __builtin_rint(t);
+    const double c = r < 127.0 ? (r > -127.0 ? r : -127.0) : 127.0;
+    return inv > 0.0 ? (int)c : 0;
+}
+__device__ __forceinline__ uint32_t int8_pack4(int a, int b, int c, int d) {
+    return (uint32_t)(a & 255) | (uint32_t)(b & 255) << 8 | (uint32_t)(c & 255) << 16 | (uint32_t)d << 24;
+}
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+// acc * s * c with one rounding that counts: the sum has up to 31 bits, the scales 24 each.
+__device__ __forceinline__ double int8_value(int acc, float s, float c) { return (double)acc * ((double)s * (double)c); }
+
+// silu(g) * u in 64 bits.  The activation that an expert hands to its down projection is rounded to
+// fp32 from this and then cut into codes: every kernel forms it the same way, so that a value next to
+// the border of two codes gets the same code however many tokens share the step.
+__device__ __forceinline__ float int8_hidden(double g, double u) { return (float)(g / (1.0 + exp(-g)) * u); }
+
+// largest of the wave (all lanes)
+__device__ __forceinline__ uint32_t wave_top(uint32_t v) {
+#pragma unroll
+    for (int off = 32; off; off >>= 1) {
+        const uint32_t o = (uint32_t)__shfl_xor((int)v, off, 64);
+        v = o > v ? o : v;
+    }
+    return v;
+}
+
+// ---- launches shared by the linear and the expert step ------------------------------------------------
+// x rows -> codes (row step ld bytes, columns up to the next multiple of 64 written, the tail as zero) + scales
+int int8_quantize_launch(const void* x, int dt, int64_t rows, int k, uint8_t* codes, int64_t ld, bool pad, float* scales, hipStream_t s);
+
+// One product or one gate/up pair; dense, or over the chunks of a plan (experts' own rows).
+struct Int8Product {
+    const uint8_t *w, *w2;            // tiles (w2: the up projection of a pair)
+    const float *c, *c2;              // channel scales
+    int n, kp;                        // output channels, padded columns
+    const uint8_t* q;                 // activation codes
+    int64_t ld;
+    const float* s;                   // their scales
+    int tokens;
+    void* y;
+    int ydt;
+    int64_t ldy;
+    // over a plan: chunk i covers sorted positions start .. start + count - 1 of expert `expert`
+    const int *chunk_expert, *chunk_start, *chunk_count, *n_chunks;
+    int64_t w_step;                   // bytes of one expert's matrix
+    const int* row_of;                // sorted position -> row of q (NULL: the position itself)
+    int hidden;                       // pair: store the expert's hidden activation (int8_hidden)
+};
+
+}  // namespace qmoe

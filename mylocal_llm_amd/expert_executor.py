@@ -16,6 +16,7 @@ from contextlib import contextmanager
 
 import torch
 
+from .int8_moe import Int8ExpertBank
 from .moe import DevicePackedExpertBank, moe_step
 from .quantized_linear import PackedExpertFFNInference
 
@@ -37,8 +38,8 @@ class ResidentExpertExecutor:
 
     # ---- residency -------------------------------------------------------------------------------
     def register_layer(self, layer_id, bank):
-        if not isinstance(bank, DevicePackedExpertBank):
-            raise TypeError("a layer's experts are registered as one DevicePackedExpertBank")
+        if not isinstance(bank, (DevicePackedExpertBank, Int8ExpertBank)):
+            raise TypeError("a layer's experts are registered as one DevicePackedExpertBank or Int8ExpertBank")
         if (bank.d_model, bank.d_ff) != (self.d_model, self.d_ff):
             raise ValueError("Executor dimensions do not match MoE tensors")
         self.banks[int(layer_id)] = bank

@@ -16,6 +16,8 @@ import numpy as np
 import torch
 
 from . import _lib
+from .int8_linear import Int8Weight
+from .int8_moe import Int8ExpertBank, int8_moe_step
 from .quantized_linear import (
     DevicePackedGGUFWeight, _FORMAT_ID, _TORCH_DTYPE_ID, _ptr, _stream, _upload_bytes, packed_to_device,
 )
@@ -201,7 +203,13 @@ def moe_step(hidden, bank, top_k, *, logits=None, weights=None, ids=None, shared
     nothing (of a repeated expert the first slot counts).  With ``check_routing`` the step's status
     word is read back afterwards (one synchronisation) and such ids raise ``ValueError``, where the
     reference hands them to its general dispatcher (mini_llm/ops/device_expert_plan.py:183-186).
+
+    An ``Int8ExpertBank`` (with ``shared`` a triple of ``Int8Weight``) makes it ``int8_moe.int8_moe_step``.
     """
+    if isinstance(bank, Int8ExpertBank):
+        return int8_moe_step(hidden, bank, top_k, logits=logits, weights=weights, ids=ids, shared=shared, shared_gate=shared_gate,
+                             floor=floor, renormalize=renormalize, out_dtype=out_dtype, return_routing=return_routing,
+                             residual=residual, check_routing=check_routing)
     if not isinstance(hidden, torch.Tensor) or not hidden.is_cuda or hidden.dtype not in _TORCH_DTYPE_ID:
         raise TypeError("MoE hidden must be a CUDA FP16/BF16/FP32 tensor")
     if hidden.ndim != 2 or hidden.shape[1] != bank.d_model or not hidden.is_contiguous():
@@ -274,7 +282,7 @@ def moe_step(hidden, bank, top_k, *, logits=None, weights=None, ids=None, shared
 class ExpertsInference:
     """Sparse expert dispatch + ordered weighted combine.
 
-    ``expert_executor`` is either a resident ``DevicePackedExpertBank`` (the layer's experts) or an
+    ``expert_executor`` is either a resident ``DevicePackedExpertBank`` or ``Int8ExpertBank`` (the layer's experts) or an
     executor with the hooks of the reference's (mini_llm/ops/experts_inference.py:188-197:
     ``try_forward_device_plan`` for one token; this package's executor also offers
     ``try_forward_batch`` for more), e.g. ``expert_executor.ResidentExpertExecutor``.
@@ -284,7 +292,7 @@ class ExpertsInference:
         self.d_model, self.d_ff, self.n_experts = d_model, d_ff, n_experts
         self.layer_id = int(layer_id)
         self.bank = self.expert_executor = None
-        if isinstance(expert_executor, DevicePackedExpertBank):
+        if isinstance(expert_executor, (DevicePackedExpertBank, Int8ExpertBank)):
             self.set_bank(expert_executor)
         elif expert_executor is not None:
             if (expert_executor.d_model, expert_executor.d_ff) != (d_model, d_ff):
@@ -350,7 +358,7 @@ class Qwen3NextMoEInference:
 
     def __init__(self, bank, top_k, router_weight, shared, shared_gate, *, normalization_floor=2.0 ** -14):
         """router_weight: fp32 [E, D] (GGUF ffn_gate_inp orientation); shared: (gate, up, down)
-        DevicePackedGGUFWeight triple, or three dense fp32 [out, in] tensors (checkpoints that keep
+        DevicePackedGGUFWeight triple (a triple of Int8Weight with an Int8ExpertBank), or three dense fp32 [out, in] tensors (checkpoints that keep
         the shared expert in F32 / F16); shared_gate: fp32 [D]."""
         self.bank = bank
         self.top_k = int(top_k)
@@ -360,8 +368,9 @@ class Qwen3NextMoEInference:
         self.router.W_router = self._router_weight.t().contiguous()
         self.router.b_router = torch.zeros(bank.n_experts, dtype=torch.float32, device=router_weight.device)
         self.shared_is_dense = all(isinstance(w, torch.Tensor) for w in shared)
-        if not self.shared_is_dense and not all(isinstance(w, DevicePackedGGUFWeight) for w in shared):
-            raise TypeError('shared expert: three DevicePackedGGUFWeight or three dense tensors')
+        packed = Int8Weight if isinstance(bank, Int8ExpertBank) else DevicePackedGGUFWeight
+        if not self.shared_is_dense and not all(isinstance(w, packed) for w in shared):
+            raise TypeError(f'shared expert: three {packed.__name__} or three dense tensors')
         self.shared = tuple(w.to(torch.float32).contiguous() for w in shared) if self.shared_is_dense else shared
         self.shared_gate = shared_gate.to(torch.float32).contiguous()
         self.experts = ExpertsInference(bank.d_model, bank.d_ff, bank.n_experts, expert_executor=bank)
@@ -378,7 +387,7 @@ class Qwen3NextMoEInference:
         dev = torch.device('cuda', torch.cuda.current_device()) if device is None else torch.device(device)
         if expert_executor is None:
             bank = index.expert_bank(layer_id, dev)
-        elif isinstance(expert_executor, DevicePackedExpertBank):
+        elif isinstance(expert_executor, (DevicePackedExpertBank, Int8ExpertBank)):
             bank = expert_executor
         else:  # an executor holding this layer's bank (expert_executor.ResidentExpertExecutor)
             if getattr(expert_executor, 'compute_dtype', 'float32') != 'float32':
@@ -394,6 +403,8 @@ class Qwen3NextMoEInference:
         host = [index.projection(stem + name) for name in ('ffn_gate_shexp.weight', 'ffn_up_shexp.weight', 'ffn_down_shexp.weight')]
         if all(isinstance(w, PackedGGUFWeight) for w in host):
             shared = tuple(packed_to_device(w, dev) for w in host)
+            if isinstance(bank, Int8ExpertBank):
+                shared = tuple(Int8Weight.from_packed(w) for w in shared)
         else:  # any F32 / F16 projection: the shared expert runs as dense fp32 matmuls
             shared = tuple(torch.from_numpy(np.ascontiguousarray(
                 w.dequantize_reference() if isinstance(w, PackedGGUFWeight) else w, dtype=np.float32)).to(dev) for w in host)

@@ -107,6 +107,11 @@ def _check_activation(x, what):
         raise TypeError("GPU input must be FP16, BF16, or FP32")
 
 
+def _is_int8(weight):
+    from .int8_linear import Int8Weight
+    return isinstance(weight, Int8Weight)
+
+
 def _host_linear(x, weight, backend):
     """NumPy activations: host-packed weight only (quantized_linear.py:292-305)."""
     from . import native_packed_cpu
@@ -131,10 +136,16 @@ def quantized_linear(x, weight, *, block_k=512, cpu_packed_backend="reference"):
     shape ``x.shape[:-1] + (N,)`` and x's dtype, accumulated in fp32 and rounded once.
     ``block_k`` is validated as in the reference and otherwise unused.  A NumPy ``x`` (fp16 /
     fp32 / fp64) with a host ``PackedGGUFWeight`` is computed on the CPU in fp32 by the library's
-    scalar C++ (every ``cpu_packed_backend`` name selects that same code).
+    scalar C++ (every ``cpu_packed_backend`` name selects that same code).  An ``Int8Weight`` in the weight's
+    place makes it ``int8_linear``: the rows of x are quantised too.
     """
     if isinstance(x, np.ndarray):
         return _host_linear(x, weight, cpu_packed_backend)
+    if not isinstance(weight, (DevicePackedGGUFWeight, PackedGGUFWeight)) and _is_int8(weight):
+        from .int8_linear import int8_linear
+        if block_k not in (256, 512, 1024):
+            raise ValueError("block_k must be 256, 512 or 1024")
+        return int8_linear(x, weight)
     _check_activation(x, "Packed linear input")
     if x.ndim not in (2, 3):
         raise ValueError("Expected x as [M, K] or [B, T, K]")
@@ -198,7 +209,13 @@ def quantized_linear_batch(problems):
 
 
 def quantized_swiglu(x, gate, up, *, block_k=512):
-    """Compute ``SiLU(x @ gate.T) * (x @ up.T)`` in one launch; gate/up formats may differ."""
+    """Compute ``SiLU(x @ gate.T) * (x @ up.T)`` in one launch; gate/up formats may differ.  Two
+    ``Int8Weight`` matrices make it ``int8_swiglu``."""
+    if not isinstance(gate, (PackedGGUFWeight, DevicePackedGGUFWeight)) and _is_int8(gate) and _is_int8(up):
+        from .int8_linear import int8_swiglu
+        if block_k not in (256, 512, 1024):
+            raise ValueError("block_k must be 256, 512 or 1024")
+        return int8_swiglu(x, gate, up)
     if not isinstance(gate, (PackedGGUFWeight, DevicePackedGGUFWeight)) or not isinstance(
             up, (PackedGGUFWeight, DevicePackedGGUFWeight)):
         raise TypeError("gate and up must be packed GGUF weights")
