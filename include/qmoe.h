@@ -312,9 +312,9 @@ int qmoe_int8_quantize(const void* x, int x_dtype, int64_t rows, int k, void* co
  * matrix every qmoe_int8_matrix_bytes(n, k) bytes. */
 int qmoe_int8_tiles(const void* codes, int64_t matrices, int n, int k, void* tiles, void* stream);
 
-/* Bytes of workspace of the two products below (not needed for codes of k % 64 == 0 at a 16-byte
- * aligned address). */
-size_t qmoe_int8_workspace_bytes(int n, int k, int tokens);
+/* Bytes of workspace of the two products below (0: none; none is needed either for codes of
+ * k % 256 == 0 at a 16-byte aligned address). */
+size_t qmoe_int8_workspace_bytes(int n, int k, int tokens, int x_dtype);
 
 /* y[tokens, n] as above, rounded once to y_dtype.  x: contiguous [tokens, k] in fp32 / fp16 / bf16,
  * quantised on the way (x_scales ignored), or QMOE_DT_INT8 with x_scales[tokens]. */

@@ -80,7 +80,7 @@ _SIGNATURES = {
     "qmoe_int8_matrix_bytes": ([_I, _I], _SZ),
     "qmoe_int8_quantize": ([_P, _I, _I64, _I, _P, _P, _P], _I),
     "qmoe_int8_tiles": ([_P, _I64, _I, _I, _P, _P], _I),
-    "qmoe_int8_workspace_bytes": ([_I, _I, _I], _SZ),
+    "qmoe_int8_workspace_bytes": ([_I, _I, _I, _I], _SZ),
     "qmoe_int8_linear": ([_P, _P, _I, _I, _P, _I, _P, _I, _P, _I, _P, _SZ, _P], _I),
     "qmoe_int8_swiglu": ([_P, _P, _P, _P, _I, _I, _P, _I, _P, _I, _P, _I, _P, _SZ, _P], _I),
     "qmoe_int8_moe_workspace_bytes": ([_I, _I, _I, _I, _I, _I], _SZ),

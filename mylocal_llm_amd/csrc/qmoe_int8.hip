@@ -4,34 +4,106 @@
 namespace qmoe {
 
 // ---- rows -> codes + scales ------------------------------------------------------------------------------
+// One workgroup a row, NX pieces of eight values a thread in registers between the search for the largest and the
+// codes: a row is read once.  Bound by the memory for many rows, by one round trip and one meeting for a few.
+//   vec   a row starts 16-byte aligned and ends on a multiple of eight values: 16-byte loads, 8-byte stores
+//   else  neighbouring threads take neighbouring values: whole lines still, 2 or 4 bytes a thread
+template <int DT, int NX, bool VEC>
+__global__ __launch_bounds__(1024) void int8_quantize_kernel(const void* __restrict__ x, int k, uint8_t* __restrict__ codes, int64_t ld,
+                                                             int width, float* __restrict__ scales) {
+    __shared__ uint32_t tops[16];
+    const int tid = threadIdx.x, threads = blockDim.x;
+    const int64_t row = blockIdx.x;
+    const size_t base = (size_t)row * k;
+    float v[NX][8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int p = 0; p < NX; ++p) {
+        if (VEC) {
+            const int i = (p * threads + tid) * 8;
+            int8_load8<DT>(x, i < k ? base + i : base, k - i, true, v[p]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int i = (p * 8 + j) * threads + tid;
+                const float f = Elem<DT>::load(x, i < k ? base + i : base);
+                v[p][j] = i < k ? f : 0.0f;
+            }
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < NX; ++p)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { const uint32_t b = abs_bits(v[p][j]); top = b > top ? b : top; }
+    top = wave_top(top);
+    if (threads > 64) {
+        if ((tid & 63) == 0) tops[tid >> 6] = top;
+        __syncthreads();
+        for (int i = 0; i < threads / 64; ++i) top = tops[i] > top ? tops[i] : top;
+    }
+    const RowScale r(top);
+    uint8_t* const out = codes + row * ld;
+#pragma unroll
+    for (int p = 0; p < NX; ++p) {
+        if (VEC) {
+            const int i = (p * threads + tid) * 8;
+            if (i < width) *(QMOE_GLOBAL u32x2_t*)(out + i) = int8_code8(v[p], r.inv);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int i = (p * 8 + j) * threads + tid;
+                if (i < width) stg<uint8_t>(out + i, (uint8_t)int8_code(v[p][j], r.inv));
+            }
+        }
+    }
+    if (tid == 0) stg<float>(scales + row, r.s);
+}
+
+// Rows of any length: read twice.
 template <int DT>
-__global__ __launch_bounds__(256) void int8_quantize_kernel(const void* __restrict__ x, int k, uint8_t* __restrict__ codes, int64_t ld,
-                                                            int width, float* __restrict__ scales) {
-    __shared__ uint32_t tops[4];
+__global__ __launch_bounds__(1024) void int8_quantize_long_kernel(const void* __restrict__ x, int64_t k, uint8_t* __restrict__ codes,
+                                                                  int64_t ld, int64_t width, float* __restrict__ scales) {
+    __shared__ uint32_t tops[16];
+    const int tid = threadIdx.x;
     const int64_t row = blockIdx.x;
     const size_t base = (size_t)row * k;
     uint32_t top = 0;
-    for (int i = threadIdx.x; i < k; i += 256) {
+    for (int64_t i = tid; i < k; i += 1024) {
         const uint32_t b = abs_bits(Elem<DT>::load(x, base + i));
         top = b > top ? b : top;
     }
     top = wave_top(top);
-    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    if ((tid & 63) == 0) tops[tid >> 6] = top;
     __syncthreads();
-    for (int i = 0; i < 4; ++i) top = tops[i] > top ? tops[i] : top;
+    for (int i = 0; i < 16; ++i) top = tops[i] > top ? tops[i] : top;
     const RowScale r(top);
-    for (int i = threadIdx.x; i < width; i += 256)
+    for (int64_t i = tid; i < width; i += 1024)
         stg<uint8_t>(codes + row * ld + i, i < k ? (uint8_t)int8_code(Elem<DT>::load(x, base + i), r.inv) : (uint8_t)0);
-    if (threadIdx.x == 0) stg<float>(scales + row, r.s);
+    if (tid == 0) stg<float>(scales + row, r.s);
+}
+
+template <int DT> static int quantize_as(const void* x, int64_t rows, int k, uint8_t* codes, int64_t ld, int width, float* scales, hipStream_t s) {
+    const dim3 grid((unsigned)rows);
+    const int eights = (width + 7) / 8;
+    if (eights > 2048) {
+        hipLaunchKernelGGL(int8_quantize_long_kernel<DT>, grid, dim3(1024), 0, s, x, (int64_t)k, codes, ld, (int64_t)width, scales);
+        return check_launch("int8 row quantisation");
+    }
+    const bool vec = k % 8 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)codes % 8 == 0 && ld % 8 == 0;
+    const int nx = eights <= 1024 ? 1 : 2;
+    const dim3 block(((eights + nx - 1) / nx + 63) / 64 * 64);
+    if (nx == 1 && vec) hipLaunchKernelGGL((int8_quantize_kernel<DT, 1, true>), grid, block, 0, s, x, k, codes, ld, width, scales);
+    else if (nx == 1) hipLaunchKernelGGL((int8_quantize_kernel<DT, 1, false>), grid, block, 0, s, x, k, codes, ld, width, scales);
+    else if (vec) hipLaunchKernelGGL((int8_quantize_kernel<DT, 2, true>), grid, block, 0, s, x, k, codes, ld, width, scales);
+    else hipLaunchKernelGGL((int8_quantize_kernel<DT, 2, false>), grid, block, 0, s, x, k, codes, ld, width, scales);
+    return check_launch("int8 row quantisation");
 }
 
 int int8_quantize_launch(const void* x, int dt, int64_t rows, int k, uint8_t* codes, int64_t ld, bool pad, float* scales, hipStream_t s) {
-    const int width = pad ? (int)int8_cols64(k) : k;
-    const dim3 grid((unsigned)rows), block(256);
-    if (dt == QMOE_DT_F32) hipLaunchKernelGGL(int8_quantize_kernel<QMOE_DT_F32>, grid, block, 0, s, x, k, codes, ld, width, scales);
-    else if (dt == QMOE_DT_F16) hipLaunchKernelGGL(int8_quantize_kernel<QMOE_DT_F16>, grid, block, 0, s, x, k, codes, ld, width, scales);
-    else hipLaunchKernelGGL(int8_quantize_kernel<QMOE_DT_BF16>, grid, block, 0, s, x, k, codes, ld, width, scales);
-    return check_launch("int8 row quantisation");
+    const int width = pad ? (int)int8_cols256(k) : k;
+    if (dt == QMOE_DT_F32) return quantize_as<QMOE_DT_F32>(x, rows, k, codes, ld, width, scales, s);
+    if (dt == QMOE_DT_F16) return quantize_as<QMOE_DT_F16>(x, rows, k, codes, ld, width, scales, s);
+    return quantize_as<QMOE_DT_BF16>(x, rows, k, codes, ld, width, scales, s);
 }
 
 // codes given by the caller with a row step the products cannot read: copied once, tail zero
@@ -100,7 +172,7 @@ int int8_product_launch(const Int8Product& a, bool pair, int chunks, hipStream_t
 
 static size_t round256(size_t v) { return (v + 255) & ~(size_t)255; }
 
-static bool codes_as_they_are(const void* x, int k) { return k % 64 == 0 && (uintptr_t)x % 16 == 0; }
+static bool codes_as_they_are(const void* x, int k) { return k % 256 == 0 && (uintptr_t)x % 16 == 0; }
 
 static int dense(const char* who, bool pair, const void* w, const float* c, const void* w2, const float* c2, int n, int k, const void* x,
                  int xdt, const float* xs, int tokens, void* y, int ydt, void* workspace, size_t bytes, hipStream_t st) {
@@ -114,14 +186,15 @@ static int dense(const char* who, bool pair, const void* w, const float* c, cons
         (xdt != QMOE_DT_I8 && (uintptr_t)x % dtype_size(xdt)) || (uintptr_t)y % dtype_size(ydt))
         return fail(QMOE_EINVAL, "%s: misaligned pointer", who);
     if (tokens == 0) return QMOE_OK;
-    const size_t need = qmoe_int8_workspace_bytes(n, k, tokens);
+    const size_t need = qmoe_int8_workspace_bytes(n, k, tokens, xdt);
     const bool direct = xdt == QMOE_DT_I8 && codes_as_they_are(x, k);
-    if (!direct && (!workspace || (uintptr_t)workspace % 256 || bytes < need))
+    if (!direct && need && (!workspace || (uintptr_t)workspace % 256 || bytes < need))
         return fail(QMOE_EWORKSPACE, "%s: workspace must be 256-byte aligned and hold %zu bytes (got %zu)", who, need, bytes);
     Int8Product a{};
     a.w = (const uint8_t*)w; a.w2 = (const uint8_t*)w2; a.c = c; a.c2 = c2;
-    a.n = n; a.kp = (int)int8_cols64(k); a.tokens = tokens; a.y = y; a.ydt = ydt; a.ldy = n; a.ld = a.kp;
+    a.n = n; a.kp = (int)int8_cols64(k); a.tokens = tokens; a.y = y; a.ydt = ydt; a.ldy = n; a.ld = int8_cols256(k);
     a.q = (const uint8_t*)x; a.s = xs;
+    if (xdt != QMOE_DT_I8 && int8_few_fuses(tokens, k)) return int8_few_launch(a, pair, x, xdt, k, st);
     if (!direct) {
         uint8_t* q = (uint8_t*)workspace;
         a.q = q;
@@ -134,7 +207,8 @@ static int dense(const char* who, bool pair, const void* w, const float* c, cons
             if (const int rc = int8_quantize_launch(x, xdt, tokens, k, q, a.ld, true, s, st)) return rc;
         }
     }
-    return int8_product_launch(a, pair, 0, st);
+    if (tokens <= INT8_FEW_TOKENS) return int8_few_launch(a, pair, nullptr, 0, k, st);
+    return int8_gemm_launch(a, pair, st);
 }
 
 }  // namespace qmoe
@@ -170,9 +244,10 @@ int qmoe_int8_tiles(const void* codes, int64_t matrices, int n, int k, void* til
     return check_launch(who);
 }
 
-size_t qmoe_int8_workspace_bytes(int n, int k, int tokens) {
+size_t qmoe_int8_workspace_bytes(int n, int k, int tokens, int x_dtype) {
     if (n < 1 || k < 1 || tokens < 1) return 0;
-    return round256((size_t)tokens * (size_t)int8_cols64(k)) + round256((size_t)tokens * 4);
+    if (x_dtype != QMOE_DT_INT8 && int8_few_fuses(tokens, k)) return 0;
+    return round256((size_t)tokens * (size_t)int8_cols256(k)) + round256((size_t)tokens * 4);
 }
 
 int qmoe_int8_linear(const void* tiles, const float* channel_scales, int n, int k, const void* x, int x_dtype, const float* x_scales,

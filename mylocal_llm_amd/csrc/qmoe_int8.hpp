@@ -7,8 +7,8 @@
 // Weight layout ("tiles"): [N/16][K/64][lane][16] bytes, lane l of a 1 KB tile holding columns
 // 16 (l / 16) .. + 15 of row l % 16 -- the A operand of v_mfma_i32_16x16x64_i8 as a wave reads it,
 // 1 KB of consecutive memory an instruction.  Rows are padded to 16 and columns to 64 with zero
-// codes, so what an activation row holds behind its K columns never counts.  Activation codes are
-// row-major with a row step that is a multiple of 16 bytes and at least K rounded up to 64: lane l
+// codes.  Activation codes are row-major with a row step that is a multiple of 16 bytes; behind its K
+// columns a row holds zeros up to a multiple of 256 (the products of many tokens read that far).  Lane l
 // reads the B operand as the 16 bytes at column 16 (l / 16) of token l % 16.  D[i] of lane l is the
 // sum of weight row 4 (l / 16) + i and token l % 16: four neighbouring outputs of one token.
 #pragma once
@@ -23,6 +23,7 @@ static constexpr int QMOE_DT_I8 = QMOE_DT_INT8;
 
 __host__ __device__ inline int64_t int8_rows16(int64_t n) { return (n + 15) / 16 * 16; }
 __host__ __device__ inline int64_t int8_cols64(int64_t k) { return (k + 63) / 64 * 64; }
+__host__ __device__ inline int64_t int8_cols256(int64_t k) { return (k + 255) / 256 * 256; }
 inline int64_t int8_matrix_bytes(int64_t n, int64_t k) { return int8_rows16(n) * int8_cols64(k); }
 
 __device__ __forceinline__ i32x4_t mfma_i8(i32x4_t a, i32x4_t b, i32x4_t c) {
@@ -61,6 +62,28 @@ __device__ __forceinline__ uint32_t int8_pack4(int a, int b, int c, int d) {
 }
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
+__device__ __forceinline__ u32x2_t int8_code8(const float* v, double inv) {
+    int q[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = int8_code(v[j], inv);
+    return u32x2_t{int8_pack4(q[0], q[1], q[2], q[3]), int8_pack4(q[4], q[5], q[6], q[7])};
+}
+// Eight values of a row from element i (in bounds with left <= 0 too); those behind the `left` that it still has are zero.
+// fast: the address is 16-byte aligned, left is not cut within the eight and eight values are there to be read.
+template <int DT> __device__ __forceinline__ void int8_load8(const void* x, size_t i, int left, bool fast, float* v) {
+    if (fast) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float4 f = Elem<DT>::load4(x, i + 4 * h);
+            v[4 * h] = left > 0 ? f.x : 0.0f; v[4 * h + 1] = left > 0 ? f.y : 0.0f;
+            v[4 * h + 2] = left > 0 ? f.z : 0.0f; v[4 * h + 3] = left > 0 ? f.w : 0.0f;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { const float f = Elem<DT>::load(x, j < left ? i + j : i); v[j] = j < left ? f : 0.0f; }
+    }
+}
+
 // acc * s * c with one rounding that counts: the sum has up to 31 bits, the scales 24 each.
 __device__ __forceinline__ double int8_value(int acc, float s, float c) { return (double)acc * ((double)s * (double)c); }
 
@@ -80,8 +103,16 @@ __device__ __forceinline__ uint32_t wave_top(uint32_t v) {
 }
 
 // ---- launches shared by the linear and the expert step ------------------------------------------------
-// x rows -> codes (row step ld bytes, columns up to the next multiple of 64 written, the tail as zero) + scales
+// x rows -> codes (row step ld bytes; pad: zeros up to the next multiple of 256 columns) + scales
 int int8_quantize_launch(const void* x, int dt, int64_t rows, int k, uint8_t* codes, int64_t ld, bool pad, float* scales, hipStream_t s);
+
+static constexpr int INT8_FEW_TOKENS = 64;
+// Whether a product of these rows quantises them in its own workgroups, and the launch for up to 64 tokens (x: rows to
+// quantise, NULL: p.q holds codes).
+bool int8_few_fuses(int tokens, int k);
+struct Int8Product;
+int int8_few_launch(const Int8Product& p, bool pair, const void* x, int xdt, int k, hipStream_t s);
+int int8_gemm_launch(const Int8Product& a, bool pair, hipStream_t s);
 
 // One product or one gate/up pair; dense, or over the chunks of a plan (experts' own rows).
 struct Int8Product {

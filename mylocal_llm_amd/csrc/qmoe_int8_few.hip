@@ -1,0 +1,218 @@
+// Products of 8-bit codes for a few tokens: the weights are streamed once.
+//
+// A workgroup of eight waves owns RT tiles of 16 channels (of both matrices of a pair) and the whole of K;
+// wave w takes the w-th eighth of the 64-column steps (neighbouring ones: it uses the activation lines it fetches whole).  A step is one 1 KB request for each tile, already the A operand
+// of the matrix instruction, and one B operand for each 16 tokens; the eight partial sums meet in LDS once, as
+// integers, so the split changes no bit of the result.  What bounds it is the memory: an instruction multiplies
+// 1 KB of weights in 16 cycles where a CU receives 1 KB in about 100, so the idle token columns cost nothing and
+// 1..16 tokens take the same time.  Up to U requests a wave and tile are outstanding while the previous U are
+// multiplied: 64 - 128 KB a CU, beyond the 48 KB that 6 TB/s needs at 2 us.
+#include "qmoe_int8.hpp"
+
+namespace qmoe {
+
+
+struct Few8Args {
+    const uint8_t *w, *w2;
+    const float *c, *c2;
+    int n, kp, steps;       // steps = kp / 64
+    const void* x;          // fused: rows to quantise
+    int k, fast;            // columns; rows may be read 16 bytes at a time
+    const uint8_t* q;       // otherwise: codes, their row step and scales
+    int64_t ld;
+    const float* s;
+    int tokens;
+    void* y;
+    int ydt;
+};
+
+// NX > 0: every workgroup quantises the rows itself (they are few: up to NX pieces of 4096 columns of a token, eight
+// values a thread and piece, kept in registers between the search for the largest and the codes), into LDS rows
+// kp + 16 bytes apart: eight neighbouring tokens' 16-byte pieces then lie in eight different bank groups.  The rows are
+// requested before the first weights, so that waiting for them does not wait for the weights.
+template <int XDT, bool PAIR, int NX, int TT, int RT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Few8Args a) {
+    constexpr bool FUSED = NX > 0;
+    constexpr int THREADS = 64 * WAVES;
+    constexpr int NP = PAIR ? 2 : 1, NW = RT * NP, U = NW >= 8 ? 1 : 8 / NW;
+    extern __shared__ uint8_t lds[];       // [codes] and, over them at the end, [waves][NW][TT][64] partial sums
+    __shared__ uint32_t tops[FUSED ? NX * WAVES : 1];
+    __shared__ float srow[16 * TT];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, g = lane >> 4;
+    const int row_tiles = (a.n + 15) / 16;
+
+    constexpr int PIECE = THREADS * 8;
+    const int per = (a.k + PIECE - 1) / PIECE;     // pieces of a token
+    float v[FUSED ? NX : 1][8];
+    if (FUSED) {
+#pragma unroll
+        for (int p = 0; p < NX; ++p) {
+            const int t = p / per, i = (p % per) * PIECE + tid * 8, left = t < a.tokens ? a.k - i : 0;
+            int8_load8<XDT>(a.x, left > 0 ? (size_t)t * a.k + i : 0, left, a.fast, v[p]);
+        }
+    }
+
+    const uint8_t* wp[NW];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        int tile = blockIdx.x * RT + r;
+        tile = tile < row_tiles ? tile : row_tiles - 1;
+        wp[r * NP] = a.w + (int64_t)tile * a.kp * 16 + lane * 16;
+        if (PAIR) wp[r * NP + 1] = a.w2 + (int64_t)tile * a.kp * 16 + lane * 16;
+    }
+    // this wave's steps; one without a step of its own (K below 512) requests its neighbour's and multiplies none
+    const int lo = a.steps * wave / WAVES, hi = a.steps * (wave + 1) / WAVES, last = hi > lo ? hi - 1 : lo < a.steps ? lo : a.steps - 1;
+    i32x4_t wr[U][NW];
+    auto request = [&](int chunk) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int step = lo + chunk * U + u < last ? lo + chunk * U + u : last;
+#pragma unroll
+            for (int i = 0; i < NW; ++i) wr[u][i] = ldg_i32x4(wp[i] + (int64_t)step * 1024);
+        }
+    };
+    request(0);
+
+    const int stride = a.kp + 16;
+    const uint8_t* qp[TT];
+    if (FUSED) {
+#pragma unroll
+        for (int p = 0; p < NX; ++p) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { const uint32_t b = abs_bits(v[p][j]); top = b > top ? b : top; }
+            top = wave_top(top);
+            if (lane == 0) tops[p * WAVES + wave] = top;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int p = 0; p < NX; ++p) {
+            const int t = p / per, i = (p % per) * PIECE + tid * 8;
+            if (t >= a.tokens) break;
+            uint32_t top = 0;
+            for (int j = t * per * WAVES; j < (t + 1) * per * WAVES; ++j) top = tops[j] > top ? tops[j] : top;
+            const RowScale rs(top);
+            if (tid == 0) srow[t] = rs.s;
+            if (i < a.kp) *(u32x2_t*)(lds + t * stride + i) = int8_code8(v[p], rs.inv);
+        }
+        __syncthreads();
+    } else {
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+            const int row = t * 16 + col;
+            qp[t] = a.q + (int64_t)(row < a.tokens ? row : a.tokens - 1) * a.ld + g * 16;
+        }
+        if (tid < 16 * TT) srow[tid] = tid < a.tokens ? a.s[tid] : 0.0f;
+    }
+
+    i32x4_t acc[NW][TT];
+#pragma unroll
+    for (int i = 0; i < NW; ++i)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) acc[i][t] = i32x4_t{0, 0, 0, 0};
+    const int chunks = (hi - lo + U - 1) / U;
+    const uint8_t* const mine = lds + (col < a.tokens ? col : a.tokens - 1) * stride + g * 16;
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+        i32x4_t now[U][NW], b[U][TT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int step = lo + chunk * U + u < last ? lo + chunk * U + u : last;
+#pragma unroll
+            for (int t = 0; t < TT; ++t)
+                b[u][t] = FUSED ? *(const i32x4_t*)(mine + step * 64) : ldg_i32x4(qp[t] + (int64_t)step * 64);
+#pragma unroll
+            for (int i = 0; i < NW; ++i) now[u][i] = wr[u][i];
+        }
+        if (chunk + 1 < chunks) request(chunk + 1);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (lo + chunk * U + u < hi) {
+#pragma unroll
+                for (int i = 0; i < NW; ++i)
+#pragma unroll
+                    for (int t = 0; t < TT; ++t) acc[i][t] = mfma_i8(now[u][i], b[u][t], acc[i][t]);
+            }
+    }
+    if (FUSED) __syncthreads();          // the codes' place is taken by the partial sums
+    int* const part = (int*)lds;
+#pragma unroll
+    for (int i = 0; i < NW; ++i)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) *(i32x4_t*)(part + ((size_t)(wave * NW + i) * TT + t) * 256 + lane * 4) = acc[i][t];
+    __syncthreads();
+    // (token, channel) of this thread: channel fastest; the sum of channel 4 g + i and token c is value i of lane 16 g + c
+    for (int o = tid; o < a.tokens * RT * 16; o += THREADS) {
+        const int ch = o % (RT * 16), t = o / (RT * 16), r = ch >> 4, in = ch & 15;
+        const int n = blockIdx.x * RT * 16 + ch;
+        if (n >= a.n) continue;
+        const int at = (t >> 4) * 256 + ((in >> 2) * 16 + (t & 15)) * 4 + (in & 3);
+        int s0 = 0, s1 = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            s0 += part[(size_t)(w * NW + r * NP) * TT * 256 + at];
+            if (PAIR) s1 += part[(size_t)(w * NW + r * NP + 1) * TT * 256 + at];
+        }
+        const double v = int8_value(s0, srow[t], a.c[n]);
+        const float out = PAIR ? int8_hidden(v, int8_value(s1, srow[t], a.c2[n])) : (float)v;
+        store_out(a.y, a.ydt, (size_t)t * a.n + n, out);
+    }
+}
+
+template <int XDT, bool PAIR, int NX, int TT, int RT, int WAVES>
+static int few8_as(const Few8Args& a, hipStream_t s) {
+    constexpr int NW = RT * (PAIR ? 2 : 1);
+    const size_t partial = (size_t)WAVES * NW * TT * 1024, codes = NX ? (size_t)a.tokens * (a.kp + 16) : 0;
+    const size_t lds = partial > codes ? partial : codes;
+    const void* fn = (const void*)&int8_few_kernel<XDT, PAIR, NX, TT, RT, WAVES>;
+    if (lds > 64 * 1024) {
+        static bool raised[64];
+        int dev = 0;
+        (void)hipGetDevice(&dev);
+        if (dev < 0 || dev >= 64 || !raised[dev]) {
+            if (hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, 150 * 1024) != hipSuccess)
+                return fail(QMOE_ELAUNCH, "int8 product: the device refuses %zu bytes of LDS", lds);
+            if (dev >= 0 && dev < 64) raised[dev] = true;
+        }
+    }
+    hipLaunchKernelGGL((int8_few_kernel<XDT, PAIR, NX, TT, RT, WAVES>), dim3((a.n + 16 * RT - 1) / (16 * RT)), dim3(64 * WAVES), lds, s, a);
+    return check_launch("int8 product of a few tokens");
+}
+
+// Rows quantised by every workgroup: one token of up to four pieces of 4096 columns.  (Two to four tokens on the way cost
+// 20.4 us where their own launch and the product take 14.1 + 2.6 us, 4 x 14336 x 4096.)
+static int few8_pieces(int k) { return (k + 4095) / 4096; }
+bool int8_few_fuses(int tokens, int k) { return tokens == 1 && few8_pieces(k) <= 4; }
+
+template <int XDT, bool PAIR, int RT> static int few8_fused(const Few8Args& a, int waves, hipStream_t s) {
+    if (waves == 16) return few8_pieces(a.k) <= 2 ? few8_as<XDT, PAIR, 1, 1, 1, 16>(a, s) : few8_as<XDT, PAIR, 2, 1, 1, 16>(a, s);
+    return few8_pieces(a.k) == 1 ? few8_as<XDT, PAIR, 1, 1, RT, 8>(a, s) : few8_as<XDT, PAIR, 4, 1, RT, 8>(a, s);
+}
+template <bool PAIR> static int few8_codes(const Few8Args& a, int rt, int waves, hipStream_t s) {
+    if (a.tokens <= 16) return waves == 16 ? few8_as<0, PAIR, 0, 1, 1, 16>(a, s) : rt == 1 ? few8_as<0, PAIR, 0, 1, 1, 8>(a, s) : few8_as<0, PAIR, 0, 1, 2, 8>(a, s);
+    if (a.tokens <= 32) return rt == 1 ? few8_as<0, PAIR, 0, 2, 1, 8>(a, s) : few8_as<0, PAIR, 0, 2, 2, 8>(a, s);
+    return rt == 1 ? few8_as<0, PAIR, 0, 4, 1, 8>(a, s) : rt == 2 || PAIR ? few8_as<0, PAIR, 0, 4, 2, 8>(a, s) : few8_as<0, PAIR, 0, 4, PAIR ? 2 : 4, 8>(a, s);
+}
+
+int int8_few_launch(const Int8Product& p, bool pair, const void* x, int xdt, int k, hipStream_t s) {
+    Few8Args a{};
+    a.w = p.w; a.w2 = p.w2; a.c = p.c; a.c2 = p.c2; a.n = p.n; a.kp = p.kp; a.steps = p.kp / 64;
+    a.q = p.q; a.ld = p.ld; a.s = p.s; a.tokens = p.tokens; a.y = p.y; a.ydt = p.ydt;
+    // Two tiles a workgroup once they still make two workgroups a CU: fewer prologues and half the activation reads for the
+    // same weights (8192 x 4096 even, 14336 x 4096 13.4 -> 12.2 us, 151936 x 2048 67.5 -> 49.8 us at one token; 4096 x 4096
+    // 5.6 -> 6.8 us); four for more than 32 tokens and 768 tiles (64 x 14336 x 4096: 44.3 / 28.8 / 21.5 us with 1 / 2 / 4).
+    // Sixteen waves where one token's row is long and the workgroups are few (4096 x 14336: 15.9 -> 14.4 us).
+    const int tiles = (p.n + 15) / 16;
+    const int rt = tiles < 512 ? 1 : tiles >= 768 && p.tokens > 32 ? 4 : 2;
+    const int waves = x && k > 4096 && tiles < 512 ? 16 : 8;
+    if (!x) return pair ? few8_codes<true>(a, rt, waves, s) : few8_codes<false>(a, rt, waves, s);
+    a.x = x; a.k = k;
+    a.fast = (uintptr_t)x % 16 == 0 && k % 8 == 0;
+#define QMOE_FUSED(DT) (pair ? few8_fused<DT, true, 1>(a, waves, s) : rt == 1 ? few8_fused<DT, false, 1>(a, waves, s) : few8_fused<DT, false, 2>(a, waves, s))
+    if (xdt == QMOE_DT_F32) return QMOE_FUSED(QMOE_DT_F32);
+    if (xdt == QMOE_DT_F16) return QMOE_FUSED(QMOE_DT_F16);
+    return QMOE_FUSED(QMOE_DT_BF16);
+#undef QMOE_FUSED
+}
+
+}  // namespace qmoe

@@ -1,0 +1,253 @@
+// Products of 8-bit codes for many tokens, dense or over the chunks of a plan.
+//
+// A workgroup owns WN x RT tiles of 16 channels (of both matrices of a pair) by WT x TT tiles of 16 tokens; a wave RT x TT
+// of them, accumulated in registers.  The weights go from memory straight to the registers that the matrix instruction
+// reads -- their layout is the A operand, 1 KB of consecutive memory a request -- one chunk of KC columns ahead.  The
+// activations are shared by the waves: a chunk of every token's codes travels through registers to LDS, two buffers,
+// one meeting a chunk, and lies there as B operands, so that an operand is one 16-byte read a lane.  Slots are XORed
+// with the piece's number: a row's pieces, written by neighbouring lanes, fall into eight bank groups, and so do the
+// rows that neighbouring lanes read.
+#include "qmoe_int8.hpp"
+#include <type_traits>
+
+namespace qmoe {
+
+// LDS operations of this workgroup's waves before and after; requests for memory stay in flight.
+__device__ __forceinline__ void meet_lds() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+template <bool PAIR, bool HIDDEN, bool PLAN, int WN, int WT, int RT, int TT, int KC, int R>
+__global__ __launch_bounds__(64 * WN * WT) void int8_gemm_kernel(const Int8Product a, int n_blocks, int t_blocks) {
+    constexpr int THREADS = 64 * WN * WT, NP = PAIR ? 2 : 1, NW = RT * NP;
+    constexpr int ROWS = 16 * TT * WT, PIECES = KC / 16, KK = KC / 64, LOADS = ROWS * PIECES / THREADS;
+    // (four pieces a row: two rows are written by eight neighbouring lanes)
+    auto swap = [](int pc) { return KC == 64 ? 2 * (pc & 3) : pc & 7; };
+    static_assert(ROWS * PIECES % THREADS == 0 && LOADS > 0, "whole pieces a thread");
+    __shared__ __align__(16) uint8_t lds[2 * ROWS * KC];
+    __shared__ float srow[ROWS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wn = wave % WN, wt = wave / WN, col = lane & 15, g = lane >> 4;
+
+    // workgroups go round the eight XCDs: neighbours in the order below share an XCD's L2
+    const int total = n_blocks * t_blocks;
+    int id = blockIdx.x;
+    if (total % 8 == 0) id = id % 8 * (total / 8) + id / 8;
+    int bn, bt;
+    if (PLAN) { bn = id % n_blocks; bt = id / n_blocks; }
+    else {
+        // bands of up to eight token blocks, channel blocks one after the other inside a band
+        const int band = id / (8 * n_blocks), in = id % (8 * n_blocks), left = t_blocks - band * 8, high = left < 8 ? left : 8;
+        bt = band * 8 + in % high;
+        bn = in / high;
+    }
+    int first = bt * ROWS, count = a.tokens - first, expert = 0;
+    if (PLAN) {
+        if (bt >= *a.n_chunks) return;
+        expert = a.chunk_expert[bt];
+        first = a.chunk_start[bt];
+        count = a.chunk_count[bt];
+    }
+
+    const int row_tiles = (a.n + 15) / 16, steps = a.kp / 64, chunks = (a.kp + KC - 1) / KC;
+    // one uniform base a matrix, 32-bit offsets behind it (a wave's tiles lie within RT * 2 MB)
+    int tile0 = (bn * WN + wn) * RT;
+    tile0 = tile0 < row_tiles ? tile0 : row_tiles - 1;
+    const uint8_t* const w0 = a.w + (int64_t)expert * a.w_step + (int64_t)tile0 * a.kp * 16;
+    const uint8_t* const w1 = PAIR ? a.w2 + (int64_t)expert * a.w_step + (int64_t)tile0 * a.kp * 16 : nullptr;
+    uint32_t w_at[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) w_at[r] = (uint32_t)(tile0 + r < row_tiles ? r : 0) * (uint32_t)a.kp * 16u;
+    const uint8_t* const x0 = PLAN ? a.q : a.q + (int64_t)first * a.ld;
+    typename std::conditional<PLAN, int64_t, uint32_t>::type xp[LOADS];
+    int slot[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const int p = tid + i * THREADS, r = p / PIECES, pc = p % PIECES;
+        const int at = r < count ? r : 0;
+        if (PLAN) xp[i] = (int64_t)(a.row_of ? a.row_of[first + at] : first + at) * a.ld + pc * 16;
+        else xp[i] = (uint32_t)at * (uint32_t)a.ld + pc * 16u;
+        slot[i] = ((r / 16 * KK + pc / 4) * 64 + pc % 4 * 16 + (r % 16 ^ swap(pc))) * 16;
+    }
+    for (int i = tid; i < ROWS; i += THREADS) {
+        const int pos = first + (i < count ? i : 0);
+        srow[i] = a.s[PLAN && a.row_of ? a.row_of[pos] : pos];
+    }
+    i32x4_t xr[LOADS], wr[R][NW];
+    auto request_x = [&](int chunk) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) xr[i] = ldg_i32x4(x0 + (xp[i] + chunk * KC));
+    };
+    auto keep_x = [&](int buffer) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) *(i32x4_t*)(lds + buffer * (ROWS * KC) + slot[i]) = xr[i];
+    };
+    // (steps behind the last repeat it: they meet activations of zero, or nothing; what is in flight never depends on a
+    // condition)
+    auto request_w = [&](int step, i32x4_t (&w)[NW]) {
+        const int64_t at = (int64_t)(step < steps ? step : steps - 1) * 1024;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            w[r * NP] = ldg_i32x4(w0 + at + (w_at[r] + lane * 16u));
+            if (PAIR) w[r * NP + 1] = ldg_i32x4(w1 + at + (w_at[r] + lane * 16u));
+        }
+    };
+    i32x4_t acc[NW][TT];
+#pragma unroll
+    for (int i = 0; i < NW; ++i)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) acc[i][t] = i32x4_t{0, 0, 0, 0};
+    // a lane's place in an operand for even and odd steps; everything else is a constant offset
+    const uint8_t* const mine0 = lds + wt * (TT * 16 * KC) + (g * 16 + (col ^ swap(g))) * 16;
+    const uint8_t* const mine1 = lds + wt * (TT * 16 * KC) + (g * 16 + (col ^ swap(g | 4))) * 16;
+    constexpr int TH = TT / 2;        // tokens' tiles of half a step
+    i32x4_t b[2][TH];
+    auto read_b = [&](int buffer, int half, i32x4_t (&to)[TH]) {
+        const int kk = half / 2;
+#pragma unroll
+        for (int t = 0; t < TH; ++t)
+            to[t] = *(const i32x4_t*)((kk & 1 ? mine1 : mine0) + (buffer * (ROWS * KC) + ((half % 2 * TH + t) * KK + kk) * 1024));
+    };
+    // A chunk in halves of a step: while one half is multiplied the next half's operands are read, and the last half of a
+    // chunk is multiplied behind the meeting that opens the next one.  A step's weights are requested again into the
+    // registers they leave, R steps ahead; activations are requested two chunks ahead of their use.
+    const int end = chunks - 1;
+    auto turn = [&](int c, int h) {
+        keep_x((h + 1) & 1);
+        request_x(c + 2 < end ? c + 2 : end);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < 2 * KK; ++j) {
+            if (j + 1 < 2 * KK) read_b(h & 1, j + 1, b[(j + 1) & 1]);
+            else {
+                meet_lds();
+                read_b((h + 1) & 1, 0, b[0]);
+            }
+            i32x4_t(&w)[NW] = wr[(h * KK + j / 2) % R];
+#pragma unroll
+            for (int t = 0; t < TH; ++t)
+#pragma unroll
+                for (int i = 0; i < NW; ++i) acc[i][j % 2 * TH + t] = mfma_i8(w[i], b[j & 1][t], acc[i][j % 2 * TH + t]);
+            if (j & 1) request_w(c * KK + j / 2 + R, w);
+            __builtin_amdgcn_sched_barrier(0);     // (the scheduler would gather the requests behind the products)
+        }
+    };
+    constexpr int ROUND = R / KK > 2 ? R / KK : 2;       // chunks after which ring and buffers are back where they were
+    static_assert(ROUND % 2 == 0 && ROUND * KK % R == 0, "a round turns both rings whole");
+    request_x(0);
+    keep_x(0);
+    request_x(1 < end ? 1 : end);
+#pragma unroll
+    for (int r = 0; r < R; ++r) request_w(r, wr[r]);
+    meet_lds();
+    read_b(0, 0, b[0]);
+    // whole rounds without a condition inside: one would make the compiler move registers that are still on their way, and
+    // wait for them
+    int c0 = 0;
+    for (; c0 + ROUND <= chunks; c0 += ROUND)
+#pragma unroll
+        for (int h = 0; h < ROUND; ++h) turn(c0 + h, h);
+#pragma unroll
+    for (int h = 0; h + 1 < ROUND; ++h)
+        if (c0 + h < chunks) turn(c0 + h, h);
+    // D[j] of a lane: channel 4 g + j of the tile, token col.  The type is decided once, not for each value: the unrolled
+    // code runs once a workgroup, and its size is its time.
+    auto value = [&](int i, int t, int j, float s, double c, double c2) -> float {
+        const double y = (double)acc[i * NP][t][j] * ((double)s * c);
+        if (!PAIR) return (float)y;
+        const double u = (double)acc[i * NP + 1][t][j] * ((double)s * c2);
+        return HIDDEN ? int8_hidden(y, u) : silu_mul((float)y, (float)u);
+    };
+    const int n0 = (bn * WN + wn) * RT * 16 + 4 * g;
+    double c[RT][4], c2[RT][4];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int n = n0 + i * 16 + j;
+            const int64_t ch = (int64_t)expert * a.n + (n < a.n ? n : a.n - 1);
+            c[i][j] = ldg<float>(a.c + ch);
+            if (PAIR) c2[i][j] = ldg<float>(a.c2 + ch);
+        }
+    // 16-bit results in fp32: three roundings of 2^-24 in front of one of 2^-9 or 2^-12, a quarter of the instructions
+    auto value32 = [&](int i, int t, int j, float s) -> float {
+        const float y = (float)acc[i * NP][t][j] * (s * (float)c[i][j]);
+        if (!PAIR) return y;
+        return silu_mul(y, (float)acc[i * NP + 1][t][j] * (s * (float)c2[i][j]));
+    };
+    auto store16 = [&](auto bits) {
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+            const int r = (wt * TT + t) * 16 + col;
+            const float s = srow[r];
+            uint16_t* const y = (uint16_t*)a.y + (size_t)(first + r) * a.ldy + n0;
+            if (r < count) {
+#pragma unroll
+                for (int i = 0; i < RT; ++i)
+                    *(QMOE_GLOBAL u32x2_t*)(y + i * 16) = u32x2_t{bits(value32(i, t, 0, s)) | bits(value32(i, t, 1, s)) << 16,
+                                                                  bits(value32(i, t, 2, s)) | bits(value32(i, t, 3, s)) << 16};
+            }
+        }
+    };
+    const bool whole = ((bn * WN + wn) * RT + RT) * 16 <= a.n && a.ldy % 4 == 0 && (uintptr_t)a.y % 16 == 0;
+    if (whole && a.ydt == QMOE_DT_F32) {
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+            const int r = (wt * TT + t) * 16 + col;
+            const float s = srow[r];
+            float* const y = (float*)a.y + (size_t)(first + r) * a.ldy + n0;
+            if (r < count) {
+#pragma unroll
+                for (int i = 0; i < RT; ++i)
+                    stg<float4>(y + i * 16, make_float4(value(i, t, 0, s, c[i][0], c2[i][0]), value(i, t, 1, s, c[i][1], c2[i][1]),
+                                                        value(i, t, 2, s, c[i][2], c2[i][2]), value(i, t, 3, s, c[i][3], c2[i][3])));
+            }
+        }
+    } else if (whole && a.ydt == QMOE_DT_BF16) {
+        store16([](float v) -> uint32_t { return __builtin_bit_cast(uint16_t, (__bf16)v); });
+    } else if (whole) {
+        store16([](float v) -> uint32_t { return __half_as_ushort(__float2half_rn(v)); });
+    } else {
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+            const int r = (wt * TT + t) * 16 + col;
+            if (r >= count) continue;
+            const float s = srow[r];
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (n0 + i * 16 + j < a.n) store_out(a.y, a.ydt, (size_t)(first + r) * a.ldy + n0 + i * 16 + j, value(i, t, j, s, c[i][j], c2[i][j]));
+        }
+    }
+}
+
+template <bool PAIR, bool HIDDEN, bool PLAN, int WN, int WT, int RT, int TT, int KC, int R>
+static int gemm8_as(const Int8Product& a, int chunks, hipStream_t s) {
+    const int nb = (a.n + 16 * WN * RT - 1) / (16 * WN * RT), tb = PLAN ? chunks : (a.tokens + 16 * WT * TT - 1) / (16 * WT * TT);
+    if ((int64_t)nb * tb > INT32_MAX) return fail(QMOE_EUNSUPPORTED, "int8 product: %d x %d blocks exceed a launch; split the tokens", nb, tb);
+    hipLaunchKernelGGL((int8_gemm_kernel<PAIR, HIDDEN, PLAN, WN, WT, RT, TT, KC, R>), dim3(nb * tb), dim3(64 * WN * WT), 0, s, a, nb, tb);
+    return check_launch("int8 product");
+}
+
+// The largest tile that still gives nearly every CU a workgroup (us; 256 x 256 of eight waves / 256 channels x 64 tokens /
+// 64 x 64, activations quantised on the way): 4096 tokens x 14336 x 4096 298 / 309 / 400, 1024 x 4096 x 4096 70 / 34 / 37,
+// 512 x 14336 x 4096 69 / 48 / 55, 128 x 4096 x 4096 57 / 29 / 15.
+int int8_gemm_launch(const Int8Product& a, bool pair, hipStream_t s) {
+    auto blocks = [&](int channels, int tokens) {
+        return (int64_t)((a.n + channels - 1) / channels) * ((a.tokens + tokens - 1) / tokens);
+    };
+    static constexpr int ENOUGH = 224;
+    if (pair) {
+        if (blocks(128, 256) >= ENOUGH) return gemm8_as<true, false, false, 4, 2, 2, 8, 128, 4>(a, 0, s);
+        if (blocks(128, 64) >= ENOUGH) return gemm8_as<true, false, false, 4, 1, 2, 4, 128, 4>(a, 0, s);
+        return gemm8_as<true, false, false, 4, 1, 1, 2, 256, 8>(a, 0, s);
+    }
+    if (blocks(256, 256) >= ENOUGH) return gemm8_as<false, false, false, 4, 2, 4, 8, 128, 4>(a, 0, s);
+    if (blocks(256, 64) >= ENOUGH) return gemm8_as<false, false, false, 4, 1, 4, 4, 128, 4>(a, 0, s);
+    return gemm8_as<false, false, false, 4, 1, 1, 4, 256, 8>(a, 0, s);
+}
+
+}  // namespace qmoe

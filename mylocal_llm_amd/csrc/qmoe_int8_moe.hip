@@ -169,14 +169,14 @@ static Int8MoeLayout int8_moe_layout(int tokens, int k, int n_experts, int d, in
     w.chunk_start = take((size_t)w.max_chunks * 4);
     w.chunk_count = take((size_t)w.max_chunks * 4);
     w.n_chunks = take(4);
-    w.q = take(t * int8_cols64(d));
+    w.q = take(t * int8_cols256(d));
     w.s = take(t * 4);
     w.h = take(a * f * 4);
-    w.hq = take(a * int8_cols64(f));
+    w.hq = take(a * int8_cols256(f));
     w.hs = take(a * 4);
     w.terms = take(a * d * 4);
     w.sh = take(fs ? t * fs * 4 : 0);
-    w.shq = take(fs ? t * int8_cols64(fs) : 0);
+    w.shq = take(fs ? t * int8_cols256(fs) : 0);
     w.shs = take(fs ? t * 4 : 0);
     w.shared_out = take(fs ? t * d * 4 : 0);
     w.total = at;
@@ -205,11 +205,11 @@ static int int8_moe_impl(const qmoe_int8_moe_args& m, char* ws, const Int8MoeLay
                        (int*)(ws + L.pos_of), (int*)(ws + L.chunk_expert), (int*)(ws + L.chunk_start), (int*)(ws + L.chunk_count),
                        (int*)(ws + L.n_chunks), m.status_out);
     if ((rc = check_launch("int8 plan"))) return rc;
-    const int64_t dp = int8_cols64(d), fp = int8_cols64(f);
+    const int64_t dp = int8_cols256(d), fp = int8_cols256(f);
     if ((rc = int8_quantize_launch(m.hidden, m.hidden_dtype, t, d, (uint8_t*)(ws + L.q), dp, true, (float*)(ws + L.s), s))) return rc;
     Int8Product p{};
     p.w = (const uint8_t*)m.gate; p.w2 = (const uint8_t*)m.up; p.c = m.gate_scales; p.c2 = m.up_scales;
-    p.n = f; p.kp = (int)dp; p.w_step = int8_matrix_bytes(f, d);
+    p.n = f; p.kp = (int)int8_cols64(d); p.w_step = int8_matrix_bytes(f, d);
     p.q = (const uint8_t*)(ws + L.q); p.ld = dp; p.s = (const float*)(ws + L.s);
     p.y = ws + L.h; p.ydt = QMOE_DT_F32; p.ldy = f; p.hidden = 1; p.tokens = t;
     p.chunk_expert = (const int*)(ws + L.chunk_expert); p.chunk_start = (const int*)(ws + L.chunk_start);
@@ -218,19 +218,19 @@ static int int8_moe_impl(const qmoe_int8_moe_args& m, char* ws, const Int8MoeLay
     if ((rc = int8_product_launch(p, true, L.max_chunks, s))) return rc;
     if ((rc = int8_quantize_launch(ws + L.h, QMOE_DT_F32, a, f, (uint8_t*)(ws + L.hq), fp, true, (float*)(ws + L.hs), s))) return rc;
     Int8Product q = p;
-    q.w = (const uint8_t*)m.down; q.c = m.down_scales; q.n = d; q.kp = (int)fp; q.w_step = int8_matrix_bytes(d, f);
+    q.w = (const uint8_t*)m.down; q.c = m.down_scales; q.n = d; q.kp = (int)int8_cols64(f); q.w_step = int8_matrix_bytes(d, f);
     q.q = (const uint8_t*)(ws + L.hq); q.ld = fp; q.s = (const float*)(ws + L.hs); q.y = ws + L.terms; q.ldy = d; q.hidden = 0;
     q.row_of = nullptr;
     if ((rc = int8_product_launch(q, false, L.max_chunks, s))) return rc;
     if (fs) {
-        const int64_t fsp = int8_cols64(fs);
+        const int64_t fsp = int8_cols256(fs);
         Int8Product g{};
         g.w = (const uint8_t*)m.shared_gate_w; g.w2 = (const uint8_t*)m.shared_up_w; g.c = m.shared_gate_scales; g.c2 = m.shared_up_scales;
-        g.n = fs; g.kp = (int)dp; g.q = p.q; g.ld = dp; g.s = p.s; g.tokens = t; g.y = ws + L.sh; g.ydt = QMOE_DT_F32; g.ldy = fs; g.hidden = 1;
+        g.n = fs; g.kp = p.kp; g.q = p.q; g.ld = dp; g.s = p.s; g.tokens = t; g.y = ws + L.sh; g.ydt = QMOE_DT_F32; g.ldy = fs; g.hidden = 1;
         if ((rc = int8_product_launch(g, true, 0, s))) return rc;
         if ((rc = int8_quantize_launch(ws + L.sh, QMOE_DT_F32, t, fs, (uint8_t*)(ws + L.shq), fsp, true, (float*)(ws + L.shs), s))) return rc;
         Int8Product o{};
-        o.w = (const uint8_t*)m.shared_down_w; o.c = m.shared_down_scales; o.n = d; o.kp = (int)fsp;
+        o.w = (const uint8_t*)m.shared_down_w; o.c = m.shared_down_scales; o.n = d; o.kp = (int)int8_cols64(fs);
         o.q = (const uint8_t*)(ws + L.shq); o.ld = fsp; o.s = (const float*)(ws + L.shs); o.tokens = t; o.y = ws + L.shared_out;
         o.ydt = QMOE_DT_F32; o.ldy = d;
         if ((rc = int8_product_launch(o, false, 0, s))) return rc;

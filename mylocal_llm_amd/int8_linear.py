@@ -7,6 +7,8 @@ tokens.  The reference keeps activations in floating point (mini_llm/ops/quantiz
 these operators stand beside ``quantized_linear`` / ``quantized_swiglu``, which take an ``Int8Weight``
 wherever they take a packed GGUF weight.
 """
+from functools import lru_cache
+
 import torch
 
 from . import _lib
@@ -16,13 +18,27 @@ MAX_K = 131071            # 128 * 128 * K stays inside int32
 _INT8 = 3                 # QMOE_DT_INT8
 
 
-def _raw_stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+def _call(device, function, *args):
+    """``function(*args, stream)`` on ``device``'s current stream, with that device current; its status."""
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        return function(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return function(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def _on(device):
-    """Context in which ``device`` is the current device (nothing to do where it already is)."""
-    return torch.cuda.device(device)
+@lru_cache(maxsize=4096)
+def _workspace_bytes(n, k, tokens, x_dtype):
+    return _lib.load().qmoe_int8_workspace_bytes(n, k, tokens, x_dtype)
+
+
+def _workspace(x, n, k, tokens, x_dtype):
+    """(tensor or None, address, bytes) of a product's scratch; codes that the kernels read as they are need none."""
+    nbytes = _workspace_bytes(n, k, tokens, x_dtype)
+    if not nbytes or (x_dtype == _INT8 and k % 256 == 0 and x.data_ptr() % 16 == 0):
+        return None, None, 0
+    work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    return work, work.data_ptr(), nbytes
 
 
 def _check_rows(x, what):
@@ -45,12 +61,11 @@ def int8_quantize(x):
     if x.dtype not in _TORCH_DTYPE_ID:
         raise TypeError("Rows to quantise must be FP16, BF16, or FP32")
     k = x.shape[-1]
-    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    codes = torch.empty_like(x, dtype=torch.int8)
+    scales = x.new_empty(x.shape[:-1], dtype=torch.float32)
     if x.numel():
-        with _on(x.device):
-            rc = _lib.load().qmoe_int8_quantize(x.data_ptr(), _TORCH_DTYPE_ID[x.dtype], x.numel() // k, k, codes.data_ptr(),
-                                                scales.data_ptr(), _raw_stream(x.device))
+        rc = _call(x.device, _lib.load().qmoe_int8_quantize, x.data_ptr(), _TORCH_DTYPE_ID[x.dtype], x.numel() // k, k,
+                   codes.data_ptr(), scales.data_ptr())
         if rc:
             _lib.check(rc, "Int8 quantisation")
     return codes, scales
@@ -72,9 +87,7 @@ def _tiles_of(codes, scales, dims, what):
     count = codes.shape[0] if dims == 3 else 1
     lib = _lib.load()
     tiles = torch.empty(count * lib.qmoe_int8_matrix_bytes(n, k), dtype=torch.uint8, device=codes.device)
-    with _on(codes.device):
-        rc = lib.qmoe_int8_tiles(codes.data_ptr(), count, n, k, tiles.data_ptr(), _raw_stream(codes.device))
-    _lib.check(rc, what)
+    _lib.check(_call(codes.device, lib.qmoe_int8_tiles, codes.data_ptr(), count, n, k, tiles.data_ptr()), what)
     return tiles
 
 
@@ -164,14 +177,11 @@ def int8_linear(x, weight, *, x_scales=None, out_dtype=None):
     n, k = weight.shape
     xdt, sp, odt = _activations(x, x_scales, k, weight.device, out_dtype, "Int8 linear input")
     m = x.numel() // k
-    out = torch.empty(x.shape[:-1] + (n,), dtype=odt, device=x.device)
+    out = x.new_empty((*x.shape[:-1], n), dtype=odt)
     if m:
-        lib = _lib.load()
-        nbytes = lib.qmoe_int8_workspace_bytes(n, k, m)
-        with _on(x.device):
-            work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-            rc = lib.qmoe_int8_linear(weight.tiles.data_ptr(), weight.scales.data_ptr(), n, k, x.data_ptr(), xdt, sp, m,
-                                      out.data_ptr(), _TORCH_DTYPE_ID[odt], work.data_ptr(), nbytes, _raw_stream(x.device))
+        work, at, nbytes = _workspace(x, n, k, m, xdt)
+        rc = _call(x.device, _lib.load().qmoe_int8_linear, weight.tiles.data_ptr(), weight.scales.data_ptr(), n, k, x.data_ptr(), xdt, sp,
+                   m, out.data_ptr(), _TORCH_DTYPE_ID[odt], at, nbytes)
         if rc:
             _lib.check(rc, "Int8 linear")
     return out
@@ -188,15 +198,11 @@ def int8_swiglu(x, gate, up, *, x_scales=None, out_dtype=None):
     f, k = gate.shape
     xdt, sp, odt = _activations(x, x_scales, k, gate.device, out_dtype, "Int8 SwiGLU input")
     m = x.numel() // k
-    out = torch.empty(x.shape[:-1] + (f,), dtype=odt, device=x.device)
+    out = x.new_empty((*x.shape[:-1], f), dtype=odt)
     if m:
-        lib = _lib.load()
-        nbytes = lib.qmoe_int8_workspace_bytes(f, k, m)
-        with _on(x.device):
-            work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-            rc = lib.qmoe_int8_swiglu(gate.tiles.data_ptr(), gate.scales.data_ptr(), up.tiles.data_ptr(), up.scales.data_ptr(), f, k,
-                                      x.data_ptr(), xdt, sp, m, out.data_ptr(), _TORCH_DTYPE_ID[odt], work.data_ptr(), nbytes,
-                                      _raw_stream(x.device))
+        work, at, nbytes = _workspace(x, f, k, m, xdt)
+        rc = _call(x.device, _lib.load().qmoe_int8_swiglu, gate.tiles.data_ptr(), gate.scales.data_ptr(), up.tiles.data_ptr(),
+                   up.scales.data_ptr(), f, k, x.data_ptr(), xdt, sp, m, out.data_ptr(), _TORCH_DTYPE_ID[odt], at, nbytes)
         if rc:
             _lib.check(rc, "Int8 SwiGLU")
     return out

@@ -7,14 +7,20 @@ expert).  ``moe_step`` hands a call with an ``Int8ExpertBank`` over to it, so ``
 ``Qwen3NextMoEInference`` and ``ResidentExpertExecutor`` take such banks as they take packed ones.
 """
 import ctypes
+from functools import lru_cache
 
 import torch
 
 from . import _lib
-from .int8_linear import Int8Weight, _codes_of, _on, _raw_stream, _tiles_of, int8_quantize
+from .int8_linear import Int8Weight, _call, _codes_of, _tiles_of, int8_quantize
 from .quantized_linear import _TORCH_DTYPE_ID
 
 _STEP_TOKENS = 4096       # tokens a call works on at a time: bounds the workspace of long prompts
+
+
+@lru_cache(maxsize=4096)
+def _workspace_bytes(*sizes):
+    return _lib.load().qmoe_int8_moe_workspace_bytes(*sizes)
 
 
 class Int8ExpertBank:
@@ -42,6 +48,11 @@ class Int8ExpertBank:
         self.gate_scales, self.up_scales, self.down_scales = scales
         self.n_experts, self.d_model, self.d_ff = e, d, f
         self.device = tiles[0].device
+        # the step's argument struct with what never changes filled in; a call copies it
+        a = self._args = _lib.Int8MoeArgs()
+        a.gate, a.up, a.down = (m.data_ptr() for m in tiles)
+        a.gate_scales, a.up_scales, a.down_scales = (m.data_ptr() for m in scales)
+        a.n_experts, a.d_model, a.d_ff = e, d, f
 
     @classmethod
     def from_packed(cls, bank):
@@ -127,7 +138,7 @@ def int8_moe_step(hidden, bank, top_k, *, logits=None, weights=None, ids=None, s
     t, k = hidden.shape[0], int(top_k)
     if not 1 <= k <= min(32, e) or e > 4096:
         raise NotImplementedError("the step covers at most 4096 experts and 1 <= top_k <= min(32, experts)")
-    args = _lib.Int8MoeArgs()
+    args = _lib.Int8MoeArgs.from_buffer_copy(bank._args)
     lg = iw = ii = rs = None
     if logits is not None:
         lg = _given(logits, torch.float32, (t, e), device, "router logits")
@@ -154,41 +165,34 @@ def int8_moe_step(hidden, bank, top_k, *, logits=None, weights=None, ids=None, s
         args.d_ff_shared = fs
         if shared_gate is not None:
             args.shared_gate = _given(shared_gate, torch.float32, (d,), device, "shared_gate")
-    out = torch.empty((t, d), dtype=out_dtype, device=device)
-    out_w = torch.empty((t, k), dtype=torch.float32, device=device) if return_routing else None
-    out_i = torch.empty((t, k), dtype=torch.int64, device=device) if return_routing else None
+    out = hidden.new_empty((t, d), dtype=out_dtype)
+    out_w = hidden.new_empty((t, k), dtype=torch.float32) if return_routing else None
+    out_i = hidden.new_empty((t, k), dtype=torch.int64) if return_routing else None
     if t == 0:
         return (out, out_w, out_i) if return_routing else out
-    lib = _lib.load()
     step = min(t, _STEP_TOKENS)
-    nbytes = lib.qmoe_int8_moe_workspace_bytes(step, k, e, d, f, fs)
-    args.hidden_dtype, args.out_dtype = _TORCH_DTYPE_ID[hidden.dtype], _TORCH_DTYPE_ID[out_dtype]
-    args.top_k, args.n_experts, args.d_model, args.d_ff = k, e, d, f
+    nbytes = _workspace_bytes(step, k, e, d, f, fs)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    status = torch.zeros(1, dtype=torch.int32, device=device) if check_routing else None
+    args.hidden_dtype, args.out_dtype, args.top_k = _TORCH_DTYPE_ID[hidden.dtype], _TORCH_DTYPE_ID[out_dtype], k
     args.floor_value, args.renormalize = float(floor), int(bool(renormalize))
-    args.gate, args.up, args.down = bank.gate_tiles.data_ptr(), bank.up_tiles.data_ptr(), bank.down_tiles.data_ptr()
-    args.gate_scales, args.up_scales, args.down_scales = (
-        bank.gate_scales.data_ptr(), bank.up_scales.data_ptr(), bank.down_scales.data_ptr())
-    with _on(device):
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        status = torch.zeros(1, dtype=torch.int32, device=device) if check_routing else None
-        stream = _raw_stream(device)
-        hp, op = hidden.data_ptr(), out.data_ptr()
-        for lo in range(0, t, step):
-            args.tokens = min(step, t - lo)
-            args.hidden, args.out = hp + lo * d * hidden.element_size(), op + lo * d * out.element_size()
-            if lg is not None:
-                args.logits = lg + lo * e * 4
-            else:
-                args.in_weights, args.in_ids = iw + lo * k * 4, ii + lo * k * 8
-            if rs is not None:
-                args.residual = rs + lo * d * 4
-            if return_routing:
-                args.out_weights, args.out_ids = out_w.data_ptr() + lo * k * 4, out_i.data_ptr() + lo * k * 8
-            if status is not None:
-                args.status_out = status.data_ptr()
-            rc = lib.qmoe_int8_moe_forward(ctypes.byref(args), workspace.data_ptr(), nbytes, stream)
-            if rc:
-                _lib.check(rc, "Int8 MoE step")
+    if status is not None:
+        args.status_out = status.data_ptr()
+    function = _lib.load().qmoe_int8_moe_forward
+    for lo in range(0, t, step):
+        args.tokens = min(step, t - lo)
+        args.hidden, args.out = hidden.data_ptr() + lo * d * hidden.element_size(), out.data_ptr() + lo * d * out.element_size()
+        if lg is not None:
+            args.logits = lg + lo * e * 4
+        else:
+            args.in_weights, args.in_ids = iw + lo * k * 4, ii + lo * k * 8
+        if rs is not None:
+            args.residual = rs + lo * d * 4
+        if return_routing:
+            args.out_weights, args.out_ids = out_w.data_ptr() + lo * k * 4, out_i.data_ptr() + lo * k * 8
+        rc = _call(device, function, ctypes.byref(args), workspace.data_ptr(), nbytes)
+        if rc:
+            _lib.check(rc, "Int8 MoE step")
     if status is not None:
         bits = int(status.item())
         if bits:

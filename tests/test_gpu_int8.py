@@ -455,12 +455,12 @@ def test_rows_behind_the_output_are_left_alone(cuda):
     t, n, k = 19, 70, 200
     x, weight = rows(t, k, 3), Int8Weight(*matrix(n, k, 4))
     out = torch.full((t + 2, n), 7.0, device=cuda)
-    need = lib.qmoe_int8_workspace_bytes(n, k, t)
+    need = lib.qmoe_int8_workspace_bytes(n, k, t, 0)
     work = torch.full((need + 512,), 123, dtype=torch.uint8, device=cuda)
     for m in (1, 5, 16, t):
         out.fill_(7.0)
         rc = lib.qmoe_int8_linear(weight.tiles.data_ptr(), weight.scales.data_ptr(), n, k, x.data_ptr(), 0, None, m, out[1].data_ptr(), 0,
-                                  work[256:].data_ptr(), lib.qmoe_int8_workspace_bytes(n, k, m), torch.cuda.current_stream().cuda_stream)
+                                  work[256:].data_ptr(), lib.qmoe_int8_workspace_bytes(n, k, m, 0), torch.cuda.current_stream().cuda_stream)
         assert rc == 0
         torch.cuda.synchronize()
         assert out[0].eq(7).all() and out[1 + m:].eq(7).all() and torch.equal(out[1:1 + m], int8_linear(x[:m], weight))

@@ -29,7 +29,7 @@ def test_linear_refuses_before_any_launch():
     assert linear(lib, xdt=7) == 1 and linear(lib, ydt=3) == 1
     assert linear(lib, xdt=3) == 1 and b"scales" in lib.qmoe_last_error()
     assert linear(lib, tiles=FAKE + 8) == 1 and linear(lib, x=FAKE + 2) == 1 and linear(lib, y=FAKE + 1) == 1
-    assert linear(lib, ws=None) == 4 and linear(lib, ws=FAKE + 16) == 4 and linear(lib, bytes=64) == 4
+    assert linear(lib, t=2, ws=None) == 4 and linear(lib, t=2, ws=FAKE + 16) == 4 and linear(lib, t=2, bytes=64) == 4
     assert linear(lib, t=0) == 0
 
 
@@ -48,8 +48,9 @@ def test_sizes():
     lib = _lib.load()
     assert lib.qmoe_int8_matrix_bytes(1, 1) == 16 * 64 and lib.qmoe_int8_matrix_bytes(17, 65) == 32 * 128 and lib.qmoe_int8_matrix_bytes(0, 4) == 0
     assert lib.qmoe_int8_matrix_bytes(70000, 65536) == 70000 * 65536
-    a, b = lib.qmoe_int8_workspace_bytes(64, 100, 3), lib.qmoe_int8_workspace_bytes(64, 100, 30)
-    assert 0 < a < b and a % 256 == b % 256 == 0 and lib.qmoe_int8_workspace_bytes(64, 100, 0) == 0
+    a, b = lib.qmoe_int8_workspace_bytes(64, 100, 3, 0), lib.qmoe_int8_workspace_bytes(64, 100, 30, 2)
+    assert 0 < a < b and a % 256 == b % 256 == 0 and lib.qmoe_int8_workspace_bytes(64, 100, 0, 0) == 0
+    assert lib.qmoe_int8_workspace_bytes(64, 100, 1, 0) == 0 and lib.qmoe_int8_workspace_bytes(64, 100, 1, 3) > 0
     m = [lib.qmoe_int8_moe_workspace_bytes(t, 10, 512, 2048, 512, 2048) for t in (1, 16, 4096)]
     assert 0 < m[0] < m[1] < m[2] and lib.qmoe_int8_moe_workspace_bytes(1, 0, 4, 4, 4, 0) == 0
 
