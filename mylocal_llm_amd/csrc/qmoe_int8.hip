@@ -47,12 +47,12 @@ __global__ __launch_bounds__(1024) void int8_quantize_kernel(const void* __restr
     for (int p = 0; p < NX; ++p) {
         if (VEC) {
             const int i = (p * threads + tid) * 8;
-            if (i < width) *(QMOE_GLOBAL u32x2_t*)(out + i) = int8_code8(v[p], r.inv);
+            if (i < width) *(QMOE_GLOBAL u32x2_t*)(out + i) = int8_code8(v[p], r);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int i = (p * 8 + j) * threads + tid;
-                if (i < width) stg<uint8_t>(out + i, (uint8_t)int8_code(v[p][j], r.inv));
+                if (i < width) stg<uint8_t>(out + i, int8_code(v[p][j], r));
             }
         }
     }
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(1024) void int8_quantize_long_kernel(const void* __
     for (int i = 0; i < 16; ++i) top = tops[i] > top ? tops[i] : top;
     const RowScale r(top);
     for (int64_t i = tid; i < width; i += 1024)
-        stg<uint8_t>(codes + row * ld + i, i < k ? (uint8_t)int8_code(Elem<DT>::load(x, base + i), r.inv) : (uint8_t)0);
+        stg<uint8_t>(codes + row * ld + i, i < k ? int8_code(Elem<DT>::load(x, base + i), r) : (uint8_t)0);
     if (tid == 0) stg<float>(scales + row, r.s);
 }
 

@@ -12,7 +12,7 @@
 // reads the B operand as the 16 bytes at column 16 (l / 16) of token l % 16.  D[i] of lane l is the
 // sum of weight row 4 (l / 16) + i and token l % 16: four neighbouring outputs of one token.
 #pragma once
-#include "qmoe_common.hpp"
+#include "qmoe_router.hpp"
 
 namespace qmoe {
 
@@ -31,43 +31,67 @@ __device__ __forceinline__ i32x4_t mfma_i8(i32x4_t a, i32x4_t b, i32x4_t c) {
 }
 __device__ __forceinline__ i32x4_t ldg_i32x4(const void* p) { return *(const QMOE_GLOBAL i32x4_t*)p; }
 
-// The scale of a row and what its codes are made with.  `top` is the largest |x| of the row as bits
-// (NaN and infinity compare above every finite value).  A row that is not finite gets the scale NaN
-// and codes of zero, so that every product of that row is NaN instead of a plausible number.
+// The scale of a row.  `top` is the largest |x| of the row as bits (NaN and infinity compare above every finite value).  A
+// row that is not finite gets the scale NaN and codes of zero, so that every product of that row is NaN instead of a
+// plausible number.
 struct RowScale {
-    float s;
-    double inv;      // 1 / s, or 0 where all codes are 0
+    float s, inv;        // inv: fl(1 / s), used where `plain`
+    bool finite, plain;  // plain: s is a normal number
     __device__ __forceinline__ explicit RowScale(uint32_t top) {
-        const bool finite = top < 0x7F800000u;
+        finite = top < 0x7F800000u;
         s = finite ? __fdiv_rn(__uint_as_float(top), 127.0f) : __uint_as_float(0x7FC00000u);
-        inv = finite && s > 0.0f ? 1.0 / (double)s : 0.0;
+        plain = s >= 1.17549435e-38f;
+        inv = plain ? __fdiv_rn(1.0f, s) : 0.0f;
     }
 };
 
-// rint(x / s), halves to even, as if the quotient were exact.  x * inv is off by less than 2^-44; a
-// quotient of two fp32 values that is not exactly n + 1/2 is at least 2^-25 away from it (x / s - (2n + 1) / 2
-// = (2x - (2n + 1) s) / 2s, and the numerator is a multiple of the smaller of the two last places).
-// Rounding to multiples of 2^-40 first therefore puts every tie on the tie and moves nothing across it.
-// (an infinite x of a row without a scale would make a NaN here: the caller's row has inv = 0 and the
-// comparison below sends it to 0)
-__device__ __forceinline__ int int8_code(float x, double inv) {
-    const double snap = 6144.0;      // 1.5 * 2^12: the last place of a sum is 2^-40
-    const double t = ((double)x * inv + snap) - snap;
-    const double r = __builtin_rint(t);
-    const double c = r < 127.0 ? (r > -127.0 ? r : -127.0) : 127.0;
-    return inv > 0.0 ? (int)c : 0;
-}
-__device__ __forceinline__ uint32_t int8_pack4(int a, int b, int c, int d) {
-    return (uint32_t)(a & 255) | (uint32_t)(b & 255) << 8 | (uint32_t)(c & 255) << 16 | (uint32_t)d << 24;
-}
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
-__device__ __forceinline__ u32x2_t int8_code8(const float* v, double inv) {
-    int q[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) q[j] = int8_code(v[j], inv);
-    return u32x2_t{int8_pack4(q[0], q[1], q[2], q[3]), int8_pack4(q[4], q[5], q[6], q[7])};
+// rint(x / s), halves to even, as if the quotient were exact; inv is 1 / s in 64 bits.  x * inv is off by less than 2^-44; a
+// quotient of two fp32 values that is not exactly n + 1/2 is at least 2^-25 away from it (x / s - (2n + 1) / 2
+// = (2x - (2n + 1) s) / 2s, and the numerator is a multiple of the smaller of the two last places).  Rounding to multiples of
+// 2^-40 first therefore puts every tie on the tie and moves nothing across it.  (inv = 0: every code is 0)
+__device__ __forceinline__ int int8_code_slow(float x, double inv) {
+    const double snap = 6144.0;      // 1.5 * 2^12: the last place of a sum is 2^-40
+    const double q = __builtin_rint(((double)x * inv + snap) - snap);
+    return inv > 0.0 ? (int)(q < 127.0 ? (q > -127.0 ? q : -127.0) : 127.0) : 0;
 }
+// N values' codes as bytes.  u = x * inv + 1.5 * 2^23 in one fma holds the nearest whole number in its low bits; x * inv is
+// within 127 * 2^-24 < 2^-17 of x / s, so wherever it is no closer than 2^-16 to a half that number is the code.  The rest,
+// one wave of 512 values in thirty, is decided in 64 bits.
+template <int N> __device__ __forceinline__ void int8_codes(const float* v, const RowScale& r, uint32_t* out) {
+    const float magic = 12582912.0f;
+    uint32_t u[N];
+    float off = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const float m = __builtin_fmaf(v[j], r.inv, magic);
+        off = fmaxf(off, fabsf(__builtin_fmaf(v[j], r.inv, magic - m)));
+        u[j] = __float_as_uint(m);
+    }
+    if (__builtin_expect(__any(!r.plain || !(off <= 0.5f - 0x1p-16f)), 0)) {
+        const double inv = r.finite && r.s > 0.0f ? 1.0 / (double)r.s : 0.0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) u[j] = (uint32_t)int8_code_slow(v[j], inv);
+    }
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+        const uint32_t lo = __builtin_amdgcn_perm(u[4 * i + 1], u[4 * i], 0x0c0c0400u), hi = __builtin_amdgcn_perm(u[4 * i + 3], u[4 * i + 2], 0x04000c0cu);
+        out[i] = lo | hi;
+    }
+    if (N < 4) out[0] = u[0] & 255u;
+}
+__device__ __forceinline__ u32x2_t int8_code8(const float* v, const RowScale& r) {
+    uint32_t w[2];
+    int8_codes<8>(v, r, w);
+    return u32x2_t{w[0], w[1]};
+}
+__device__ __forceinline__ uint8_t int8_code(float v, const RowScale& r) {
+    uint32_t w;
+    int8_codes<1>(&v, r, &w);
+    return (uint8_t)w;
+}
+
 // Eight values of a row from element i (in bounds with left <= 0 too); those behind the `left` that it still has are zero.
 // fast: the address is 16-byte aligned, left is not cut within the eight and eight values are there to be read.
 template <int DT> __device__ __forceinline__ void int8_load8(const void* x, size_t i, int left, bool fast, float* v) {
@@ -92,14 +116,14 @@ __device__ __forceinline__ double int8_value(int acc, float s, float c) { return
 // the border of two codes gets the same code however many tokens share the step.
 __device__ __forceinline__ float int8_hidden(double g, double u) { return (float)(g / (1.0 + exp(-g)) * u); }
 
-// largest of the wave (all lanes)
-__device__ __forceinline__ uint32_t wave_top(uint32_t v) {
-#pragma unroll
-    for (int off = 32; off; off >>= 1) {
-        const uint32_t o = (uint32_t)__shfl_xor((int)v, off, 64);
-        v = o > v ? o : v;
-    }
-    return v;
+// largest of the wave
+__device__ __forceinline__ uint32_t wave_top(uint32_t v) { return wave_max_u32(v); }
+
+// LDS operations of this workgroup's waves before and after; requests for memory stay in flight.
+__device__ __forceinline__ void meet_lds() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 // ---- launches shared by the linear and the expert step ------------------------------------------------

@@ -94,7 +94,7 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Few8Args a) 
             for (int j = t * per * WAVES; j < (t + 1) * per * WAVES; ++j) top = tops[j] > top ? tops[j] : top;
             const RowScale rs(top);
             if (tid == 0) srow[t] = rs.s;
-            if (i < a.kp) *(u32x2_t*)(lds + t * stride + i) = int8_code8(v[p], rs.inv);
+            if (i < a.kp) *(u32x2_t*)(lds + t * stride + i) = int8_code8(v[p], rs);
         }
         __syncthreads();
     } else {

@@ -12,13 +12,6 @@
 
 namespace qmoe {
 
-// LDS operations of this workgroup's waves before and after; requests for memory stay in flight.
-__device__ __forceinline__ void meet_lds() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
-
 template <bool PAIR, bool HIDDEN, bool PLAN, int WN, int WT, int RT, int TT, int KC, int R>
 __global__ __launch_bounds__(64 * WN * WT) void int8_gemm_kernel(const Int8Product a, int n_blocks, int t_blocks) {
     constexpr int THREADS = 64 * WN * WT, NP = PAIR ? 2 : 1, NW = RT * NP;

@@ -13,6 +13,10 @@ int int8_product_launch(const Int8Product& a, bool pair, int chunks, hipStream_t
 int router_topk_impl(const float* logits, int tokens, int n, int k, float floor_value, int renorm, float* weights, int64_t* ids,
                      hipStream_t s);
 
+bool int8_step_covers(int tokens, int k, int n_experts, int d, int f, int fs);
+size_t int8_step_bytes(int tokens, int k, int f, int fs);
+int int8_step_launch(const qmoe_int8_moe_args& m, char* ws, hipStream_t s);
+
 static constexpr int PLAN8_THREADS = 256;
 static constexpr int PLAN8_GRID = 64;
 static constexpr int INT8_CHUNK = 16;         // sorted positions of one expert that a product takes at a time
@@ -183,6 +187,11 @@ static Int8MoeLayout int8_moe_layout(int tokens, int k, int n_experts, int d, in
     return w;
 }
 
+static size_t int8_moe_bytes(int tokens, int k, int n_experts, int d, int f, int fs) {
+    return int8_step_covers(tokens, k, n_experts, d, f, fs) ? int8_step_bytes(tokens, k, f, fs)
+                                                             : int8_moe_layout(tokens, k, n_experts, d, f, fs).total;
+}
+
 static int int8_moe_impl(const qmoe_int8_moe_args& m, char* ws, const Int8MoeLayout& L, hipStream_t s) {
     const int t = m.tokens, k = m.top_k, e = m.n_experts, d = m.d_model, f = m.d_ff, fs = m.d_ff_shared;
     const int a = t * k;
@@ -285,7 +294,7 @@ extern "C" {
 
 size_t qmoe_int8_moe_workspace_bytes(int tokens, int top_k, int n_experts, int d_model, int d_ff, int d_ff_shared) {
     if (tokens < 0 || top_k < 1 || n_experts < 1 || d_model < 1 || d_ff < 1 || d_ff_shared < 0) return 0;
-    return int8_moe_layout(tokens, top_k, n_experts, d_model, d_ff, d_ff_shared).total;
+    return int8_moe_bytes(tokens, top_k, n_experts, d_model, d_ff, d_ff_shared);
 }
 
 int qmoe_int8_moe_forward(const qmoe_int8_moe_args* args, void* workspace, size_t workspace_bytes, void* stream) {
@@ -293,10 +302,13 @@ int qmoe_int8_moe_forward(const qmoe_int8_moe_args* args, void* workspace, size_
     if (!args) return fail(QMOE_EINVAL, "%s: null argument struct", who);
     if (const int rc = int8_moe_check(*args)) return rc;
     if (args->tokens == 0) return QMOE_OK;
-    const Int8MoeLayout L = int8_moe_layout(args->tokens, args->top_k, args->n_experts, args->d_model, args->d_ff, args->d_ff_shared);
-    if (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < L.total)
-        return fail(QMOE_EWORKSPACE, "%s: workspace must be 256-byte aligned and hold %zu bytes (got %zu)", who, L.total, workspace_bytes);
-    return int8_moe_impl(*args, (char*)workspace, L, (hipStream_t)stream);
+    const qmoe_int8_moe_args& m = *args;
+    const size_t need = int8_moe_bytes(m.tokens, m.top_k, m.n_experts, m.d_model, m.d_ff, m.d_ff_shared);
+    if (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < need)
+        return fail(QMOE_EWORKSPACE, "%s: workspace must be 256-byte aligned and hold %zu bytes (got %zu)", who, need, workspace_bytes);
+    if (int8_step_covers(m.tokens, m.top_k, m.n_experts, m.d_model, m.d_ff, m.d_ff_shared))
+        return int8_step_launch(m, (char*)workspace, (hipStream_t)stream);
+    return int8_moe_impl(m, (char*)workspace, int8_moe_layout(m.tokens, m.top_k, m.n_experts, m.d_model, m.d_ff, m.d_ff_shared), (hipStream_t)stream);
 }
 
 }  // extern "C"
