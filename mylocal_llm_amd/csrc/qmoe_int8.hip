@@ -129,47 +129,6 @@ __global__ __launch_bounds__(256) void int8_tiles_kernel(const uint8_t* __restri
     }
 }
 
-// ---- products: one wave per 16 channels x 16 tokens ---------------------------------------------------------
-template <bool PAIR>
-__global__ __launch_bounds__(64) void int8_product_kernel(const Int8Product a) {
-    const int lane = threadIdx.x, col = lane & 15, g = lane >> 4;
-    int first = blockIdx.y * 16, count = a.tokens - first, expert = 0;
-    if (a.n_chunks) {
-        if ((int)blockIdx.y >= *a.n_chunks) return;
-        expert = a.chunk_expert[blockIdx.y];
-        first = a.chunk_start[blockIdx.y];
-        count = a.chunk_count[blockIdx.y];
-    }
-    const int pos = first + (col < count ? col : 0);
-    const int64_t row = a.row_of ? a.row_of[pos] : pos;
-    const uint8_t* q = a.q + row * a.ld + g * 16;
-    const int64_t at = (int64_t)blockIdx.x * a.kp * 16 + lane * 16 + expert * a.w_step;
-    i32x4_t acc = {0, 0, 0, 0}, acc2 = {0, 0, 0, 0};
-    for (int k = 0; k < a.kp; k += 64) {
-        const i32x4_t b = ldg_i32x4(q + k);
-        acc = mfma_i8(ldg_i32x4(a.w + at + (int64_t)k * 16), b, acc);
-        if (PAIR) acc2 = mfma_i8(ldg_i32x4(a.w2 + at + (int64_t)k * 16), b, acc2);
-    }
-    if (col >= count) return;
-    const float s = a.s[row];
-    for (int i = 0; i < 4; ++i) {
-        const int n = blockIdx.x * 16 + 4 * g + i;
-        if (n >= a.n) break;
-        const double v = int8_value(acc[i], s, a.c[(int64_t)expert * a.n + n]);
-        const size_t out = (size_t)(pos * a.ldy + n);
-        if (!PAIR) { store_out(a.y, a.ydt, out, (float)v); continue; }
-        const double u = int8_value(acc2[i], s, a.c2[(int64_t)expert * a.n + n]);
-        store_out(a.y, a.ydt, out, int8_hidden(v, u));
-    }
-}
-
-int int8_product_launch(const Int8Product& a, bool pair, int chunks, hipStream_t s) {
-    const dim3 grid((a.n + 15) / 16, a.n_chunks ? chunks : (a.tokens + 15) / 16);
-    if (pair) hipLaunchKernelGGL(int8_product_kernel<true>, grid, dim3(64), 0, s, a);
-    else hipLaunchKernelGGL(int8_product_kernel<false>, grid, dim3(64), 0, s, a);
-    return check_launch("int8 product");
-}
-
 static size_t round256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 static bool codes_as_they_are(const void* x, int k) { return k % 256 == 0 && (uintptr_t)x % 16 == 0; }

@@ -24,10 +24,11 @@ __global__ __launch_bounds__(64 * WN * WT) void int8_gemm_kernel(const Int8Produ
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wn = wave % WN, wt = wave / WN, col = lane & 15, g = lane >> 4;
 
-    // workgroups go round the eight XCDs: neighbours in the order below share an XCD's L2
-    const int total = n_blocks * t_blocks;
-    int id = blockIdx.x;
-    if (total % 8 == 0) id = id % 8 * (total / 8) + id / 8;
+    // workgroups go round the eight XCDs: each XCD takes a run of neighbours in the order below, for its L2
+    const int total = PLAN ? n_blocks * *(const QMOE_GLOBAL int*)a.n_chunks : n_blocks * t_blocks;
+    if (PLAN && (int)blockIdx.x >= total) return;
+    const int xcd = blockIdx.x % 8, share = total / 8, over = total % 8;
+    const int id = xcd * share + (xcd < over ? xcd : over) + blockIdx.x / 8;
     int bn, bt;
     if (PLAN) { bn = id % n_blocks; bt = id / n_blocks; }
     else {
@@ -38,7 +39,6 @@ __global__ __launch_bounds__(64 * WN * WT) void int8_gemm_kernel(const Int8Produ
     }
     int first = bt * ROWS, count = a.tokens - first, expert = 0;
     if (PLAN) {
-        if (bt >= *a.n_chunks) return;
         expert = a.chunk_expert[bt];
         first = a.chunk_start[bt];
         count = a.chunk_count[bt];
@@ -225,6 +225,22 @@ static int gemm8_as(const Int8Product& a, int chunks, hipStream_t s) {
     return check_launch("int8 product");
 }
 
+// A chunk of a plan holds up to `rows` sorted positions of one expert: 32, 64 or 128.
+int int8_plan_rows(int64_t assignments, int n_experts) {
+    const int64_t average = assignments / n_experts;
+    return average <= 24 ? 32 : average <= 96 ? 64 : 128;
+}
+int int8_plan_launch(const Int8Product& a, bool pair, int rows, int max_chunks, hipStream_t s) {
+    if (pair) {
+        if (rows == 32) return gemm8_as<true, true, true, 4, 1, 1, 2, 256, 8>(a, max_chunks, s);
+        if (rows == 64) return gemm8_as<true, true, true, 4, 1, 1, 4, 256, 8>(a, max_chunks, s);
+        return gemm8_as<true, true, true, 4, 1, 2, 8, 128, 4>(a, max_chunks, s);
+    }
+    if (rows == 32) return gemm8_as<false, false, true, 4, 1, 2, 2, 256, 8>(a, max_chunks, s);
+    if (rows == 64) return gemm8_as<false, false, true, 4, 1, 2, 4, 256, 8>(a, max_chunks, s);
+    return gemm8_as<false, false, true, 4, 1, 4, 8, 128, 4>(a, max_chunks, s);
+}
+
 // The largest tile that still gives nearly every CU a workgroup (us; 256 x 256 of eight waves / 256 channels x 64 tokens /
 // 64 x 64, activations quantised on the way): 4096 tokens x 14336 x 4096 298 / 309 / 400, 1024 x 4096 x 4096 70 / 34 / 37,
 // 512 x 14336 x 4096 69 / 48 / 55, 128 x 4096 x 4096 57 / 29 / 15.
@@ -233,6 +249,10 @@ int int8_gemm_launch(const Int8Product& a, bool pair, hipStream_t s) {
         return (int64_t)((a.n + channels - 1) / channels) * ((a.tokens + tokens - 1) / tokens);
     };
     static constexpr int ENOUGH = 224;
+    if (pair && a.hidden) {
+        if (blocks(128, 64) >= ENOUGH) return gemm8_as<true, true, false, 4, 1, 2, 4, 128, 4>(a, 0, s);
+        return gemm8_as<true, true, false, 4, 1, 1, 2, 256, 8>(a, 0, s);
+    }
     if (pair) {
         if (blocks(128, 256) >= ENOUGH) return gemm8_as<true, false, false, 4, 2, 2, 8, 128, 4>(a, 0, s);
         if (blocks(128, 64) >= ENOUGH) return gemm8_as<true, false, false, 4, 1, 2, 4, 128, 4>(a, 0, s);

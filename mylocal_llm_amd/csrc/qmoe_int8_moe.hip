@@ -9,104 +9,130 @@
 
 namespace qmoe {
 
-int int8_product_launch(const Int8Product& a, bool pair, int chunks, hipStream_t s);
-int router_topk_impl(const float* logits, int tokens, int n, int k, float floor_value, int renorm, float* weights, int64_t* ids,
-                     hipStream_t s);
-
 bool int8_step_covers(int tokens, int k, int n_experts, int d, int f, int fs);
 size_t int8_step_bytes(int tokens, int k, int f, int fs);
 int int8_step_launch(const qmoe_int8_moe_args& m, char* ws, hipStream_t s);
 
-static constexpr int PLAN8_THREADS = 256;
-static constexpr int PLAN8_GRID = 64;
-static constexpr int INT8_CHUNK = 16;         // sorted positions of one expert that a product takes at a time
+static constexpr int PLAN8_THREADS = 1024;
+static constexpr int PLAN8_MIN_ROWS = 32;     // of a chunk (the workspace is laid out for the most chunks there can be)
 
-// ---- plan ------------------------------------------------------------------------------------------------
-// Whether assignment a counts: its id lies in the bank and no earlier slot of its token names it.
-__device__ __forceinline__ int plan_fault(const int64_t* ids, int64_t a, int k, int n_experts) {
-    const int64_t e = ids[a];
-    if (e < 0 || e >= n_experts) return 1;
-    for (int64_t j = a - a % k; j < a; ++j)
-        if (ids[j] == e) return 2;
-    return 0;
+// ---- routing and codes of a prompt: a workgroup a token, its first wave routes ---------------------------------
+template <int XDT>
+__global__ __launch_bounds__(320) void int8_route_kernel(const void* __restrict__ x, int d, int fast, const float* __restrict__ logits,
+                                                         int n_experts, int k, float floor_value, int renorm,
+                                                         const float* __restrict__ in_weights, const int64_t* __restrict__ in_ids,
+                                                         float* __restrict__ weights, int64_t* __restrict__ ids, float* __restrict__ out_weights,
+                                                         int64_t* __restrict__ out_ids, uint8_t* __restrict__ codes, int64_t ld,
+                                                         float* __restrict__ scales) {
+    __shared__ uint32_t tops[4];
+    const int64_t t = blockIdx.x;
+    const int lane = threadIdx.x & 63, tid = (int)threadIdx.x - 64;
+    float v[8];
+    uint32_t top = 0;
+    if (tid < 0) {
+        float w = 0.0f;
+        int64_t id = 0;
+        if (logits) router_row<64>(logits + t * n_experts, n_experts, k, floor_value, renorm, w, id, [] {});
+        else if (lane < k) {
+            w = ldg<float>(in_weights + t * k + lane);
+            id = ldg<int64_t>(in_ids + t * k + lane);
+        }
+        if (lane < k) {
+            stg<float>(weights + t * k + lane, w);
+            stg<int64_t>(ids + t * k + lane, id);
+            if (out_weights) stg<float>(out_weights + t * k + lane, w);
+            if (out_ids) stg<int64_t>(out_ids + t * k + lane, id);
+        }
+    } else {
+        for (int i = tid * 8; i < d; i += 2048) {       // (the first 2048 columns stay in registers)
+            float u[8];
+            int8_load8<XDT>(x, (size_t)t * d + i, d - i, fast, u);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t b = abs_bits(u[j]);
+                top = b > top ? b : top;
+                if (i < 2048) v[j] = u[j];
+            }
+        }
+        top = wave_top(top);
+        if (lane == 0) tops[tid >> 6] = top;
+    }
+    __syncthreads();
+    if (tid < 0) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = tops[i] > top ? tops[i] : top;
+    const RowScale r(top);
+    if (tid == 0) stg<float>(scales + t, r.s);
+    for (int i = tid * 8; i < ld; i += 2048) {
+        float u[8];
+        if (i >= 2048 || i >= d) int8_load8<XDT>(x, i < d ? (size_t)t * d + i : (size_t)t * d, d - i, fast, u);
+        else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[j] = v[j];
+        }
+        *(QMOE_GLOBAL u32x2_t*)(codes + t * ld + i) = int8_code8(u, r);
+    }
 }
 
-// Every workgroup counts all assignments (LDS integer adds: the order does not matter), turns the counts into
-// positions and chunks, and ranks the assignments of its own experts, one wave an expert: ascending position is
-// ascending token.  No workgroup waits for another and the number of tokens is not bounded by a table.
+// ---- plan ------------------------------------------------------------------------------------------------
+// One workgroup groups the assignments by expert.  The place of an assignment inside its expert is the order in which the
+// adds to the expert's counter happened: it may differ from run to run, and no result depends on it, since a row's
+// products do not depend on its neighbours.  An assignment counts if its id lies in the bank and no earlier slot of its token
+// names it; the others get the position -1 and are reported.
 __global__ __launch_bounds__(PLAN8_THREADS) void int8_plan_kernel(const int64_t* __restrict__ ids, int assignments, int k, int n_experts,
-                                                                  int* __restrict__ row_of, int* __restrict__ pos_of,
+                                                                  int rows, int* __restrict__ row_of, int* __restrict__ pos_of,
                                                                   int* __restrict__ chunk_expert, int* __restrict__ chunk_start,
                                                                   int* __restrict__ chunk_count, int* __restrict__ n_chunks,
                                                                   int* __restrict__ status_out) {
-    extern __shared__ int count[];               // [experts] counts, [experts] starts, [experts] first chunks
-    __shared__ int part[2][PLAN8_THREADS];
+    extern __shared__ int count[];               // [experts] counts, [experts] starts
+    __shared__ int part[2][PLAN8_THREADS / 64];
     int* const start = count + n_experts;
-    int* const chunk0 = start + n_experts;
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     for (int e = tid; e < n_experts; e += PLAN8_THREADS) count[e] = 0;
     __syncthreads();
     int bad = 0;
-    for (int64_t a = tid; a < assignments; a += PLAN8_THREADS) {
-        const int f = plan_fault(ids, a, k, n_experts);
-        bad |= f;
-        if (!f) atomicAdd(&count[ids[a]], 1);
-        else if (blockIdx.x == 0) pos_of[a] = -1;
+    for (int a = tid; a < assignments; a += PLAN8_THREADS) {
+        const int64_t e = ldg<int64_t>(ids + a);
+        const int first = a / k * k;
+        int fault = e < 0 || e >= n_experts ? 1 : 0;
+        for (int j = first; j < a; ++j) fault |= ldg<int64_t>(ids + j) == e ? 2 : 0;
+        if (fault & 1) fault = 1;
+        bad |= fault;
+        pos_of[a] = fault ? -1 : atomicAdd(&count[e], 1);      // (the rank; its expert's start is added below)
     }
-    if (bad && blockIdx.x == 0 && status_out) atomicOr(status_out, bad);
+    if (bad && status_out) atomicOr(status_out, bad);
     __syncthreads();
-    const int per = (n_experts + PLAN8_THREADS - 1) / PLAN8_THREADS;
+    const int per = (n_experts + PLAN8_THREADS - 1) / PLAN8_THREADS, e0 = tid * per;
     int sum = 0, chunks = 0;
-    for (int e = tid * per; e < (tid + 1) * per && e < n_experts; ++e) {
-        sum += count[e];
-        chunks += (count[e] + INT8_CHUNK - 1) / INT8_CHUNK;
+    for (int e = e0; e < e0 + per && e < n_experts; ++e) { sum += count[e]; chunks += (count[e] + rows - 1) / rows; }
+    int upto = sum, cupto = chunks;              // inclusive, then exclusive prefix
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int o = __shfl_up(upto, off, 64), c = __shfl_up(cupto, off, 64);
+        if (lane >= off) { upto += o; cupto += c; }
     }
-    part[0][tid] = sum;
-    part[1][tid] = chunks;
+    if (lane == 63) { part[0][wave] = upto; part[1][wave] = cupto; }
     __syncthreads();
-    if (tid < 2) {
-        int run = 0;
-        for (int i = 0; i < PLAN8_THREADS; ++i) { const int c = part[tid][i]; part[tid][i] = run; run += c; }
-        if (tid == 1 && blockIdx.x == 0) *n_chunks = run;
-    }
-    __syncthreads();
-    sum = part[0][tid];
-    chunks = part[1][tid];
-    for (int e = tid * per; e < (tid + 1) * per && e < n_experts; ++e) {
-        start[e] = sum;
-        chunk0[e] = chunks;
-        sum += count[e];
-        chunks += (count[e] + INT8_CHUNK - 1) / INT8_CHUNK;
-    }
-    __syncthreads();
-    for (int e = blockIdx.x * (PLAN8_THREADS / 64) + (tid >> 6); e < n_experts; e += gridDim.x * (PLAN8_THREADS / 64)) {
-        const int c = count[e], s0 = start[e];
-        if (!c) continue;
-        for (int i = lane; i * INT8_CHUNK < c; i += 64) {
-            chunk_expert[chunk0[e] + i] = e;
-            chunk_start[chunk0[e] + i] = s0 + i * INT8_CHUNK;
-            chunk_count[chunk0[e] + i] = c - i * INT8_CHUNK < INT8_CHUNK ? c - i * INT8_CHUNK : INT8_CHUNK;
+    upto -= sum;
+    cupto -= chunks;
+    for (int w = 0; w < wave; ++w) { upto += part[0][w]; cupto += part[1][w]; }
+    if (tid == PLAN8_THREADS - 1) *n_chunks = cupto + chunks;
+    for (int e = e0; e < e0 + per && e < n_experts; ++e) {
+        start[e] = upto;
+        for (int at = 0; at < count[e]; at += rows) {
+            chunk_expert[cupto] = e;
+            chunk_start[cupto] = upto + at;
+            chunk_count[cupto++] = count[e] - at < rows ? count[e] - at : rows;
         }
-        int at = s0;
-        for (int64_t a0 = 0; a0 < assignments && at < s0 + c; a0 += 64) {
-            const int64_t a = a0 + lane;
-            const bool mine = a < assignments && ids[a] == e && !plan_fault(ids, a, k, n_experts);
-            const unsigned long long m = __ballot(mine);
-            if (mine) {
-                const int p = at + __popcll(m & ((1ull << lane) - 1));
-                row_of[p] = (int)(a / k);
-                pos_of[a] = p;
-            }
-            at += __popcll(m);
-        }
+        upto += count[e];
     }
-}
-
-__global__ __launch_bounds__(256) void int8_routing_copy_kernel(const float* __restrict__ w, const int64_t* __restrict__ ids, int64_t n,
-                                                                float* __restrict__ out_w, int64_t* __restrict__ out_ids) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        if (out_w && out_w != w) out_w[i] = w[i];
-        if (out_ids && out_ids != ids) out_ids[i] = ids[i];
+    __syncthreads();
+    for (int a = tid; a < assignments; a += PLAN8_THREADS) {
+        const int rank = pos_of[a];              // (written by this thread)
+        if (rank < 0) continue;
+        const int p = start[ldg<int64_t>(ids + a)] + rank;
+        pos_of[a] = p;
+        row_of[p] = a / k;
     }
 }
 
@@ -135,9 +161,16 @@ __global__ __launch_bounds__(256) void int8_combine_kernel(const float* __restri
         if (tid == 0) kept = n;
     }
     float admit = 1.0f;
+    const bool wide = d % 4 == 0 && ((uintptr_t)x | (uintptr_t)shared_gate | (uintptr_t)residual | (uintptr_t)out) % 16 == 0;
     if (shared_out && shared_gate) {
         float a = 0.0f;
-        for (int i = tid; i < d; i += 256) a += Elem<XDT>::load(x, (size_t)t * d + i) * shared_gate[i];
+        if (wide)
+            for (int i = 4 * tid; i < d; i += 1024) {
+                const float4 h = Elem<XDT>::load4(x, (size_t)t * d + i), g = ldg<float4>(shared_gate + i);
+                a += (h.x * g.x + h.y * g.y) + (h.z * g.z + h.w * g.w);
+            }
+        else
+            for (int i = tid; i < d; i += 256) a += Elem<XDT>::load(x, (size_t)t * d + i) * shared_gate[i];
         a = wave_sum(a);
         if ((tid & 63) == 0) partial[tid >> 6] = a;
         __syncthreads();
@@ -145,6 +178,38 @@ __global__ __launch_bounds__(256) void int8_combine_kernel(const float* __restri
         admit = a >= 0.0f ? 1.0f / (1.0f + expf(-a)) : expf(a) / (1.0f + expf(a));
     }
     __syncthreads();
+    if (wide) {
+        // four columns a thread; eight terms' requests leave together, the adds follow in order
+        for (int i = 4 * tid; i < d; i += 1024) {
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int j0 = 0; j0 < kept; j0 += 8) {
+                float4 v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = ldg<float4>(terms + (size_t)pos[j0 + j < kept ? j0 + j : 0] * d + i);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j0 + j < kept) {
+                        const float w = weight[j0 + j];
+                        acc.x = add_product(acc.x, v[j].x, w); acc.y = add_product(acc.y, v[j].y, w);
+                        acc.z = add_product(acc.z, v[j].z, w); acc.w = add_product(acc.w, v[j].w, w);
+                    }
+            }
+            if (shared_out) {
+                const float4 v = ldg<float4>(shared_out + (size_t)t * d + i);
+                acc.x = add_product(acc.x, v.x, admit); acc.y = add_product(acc.y, v.y, admit);
+                acc.z = add_product(acc.z, v.z, admit); acc.w = add_product(acc.w, v.w, admit);
+            }
+            if (residual) {
+                const float4 r = ldg<float4>(residual + (size_t)t * d + i);
+                acc.x = __fadd_rn(r.x, acc.x); acc.y = __fadd_rn(r.y, acc.y); acc.z = __fadd_rn(r.z, acc.z); acc.w = __fadd_rn(r.w, acc.w);
+            }
+            const float o[4] = {acc.x, acc.y, acc.z, acc.w};
+            if (odt == QMOE_DT_F32) stg<float4>((float*)out + (size_t)t * d + i, acc);
+            else
+                for (int j = 0; j < 4; ++j) store_out(out, odt, (size_t)t * d + i + j, o[j]);
+        }
+        return;
+    }
     for (int i = tid; i < d; i += 256) {
         float acc = 0.0f;
         for (int j = 0; j < kept; ++j) acc = add_product(acc, terms[(size_t)pos[j] * d + i], weight[j]);
@@ -164,7 +229,7 @@ static Int8MoeLayout int8_moe_layout(int tokens, int k, int n_experts, int d, in
     size_t at = 0;
     const size_t a = (size_t)tokens * k, t = (size_t)tokens;
     auto take = [&](size_t bytes) { const size_t here = at; at = (at + bytes + 255) & ~(size_t)255; return here; };
-    w.max_chunks = (int)(a / INT8_CHUNK + (a < (size_t)n_experts ? a : (size_t)n_experts));
+    w.max_chunks = (int)(a / PLAN8_MIN_ROWS + (a < (size_t)n_experts ? a : (size_t)n_experts));
     w.weights = take(a * 4);
     w.ids = take(a * 8);
     w.row_of = take(a * 4);
@@ -195,27 +260,25 @@ static size_t int8_moe_bytes(int tokens, int k, int n_experts, int d, int f, int
 static int int8_moe_impl(const qmoe_int8_moe_args& m, char* ws, const Int8MoeLayout& L, hipStream_t s) {
     const int t = m.tokens, k = m.top_k, e = m.n_experts, d = m.d_model, f = m.d_ff, fs = m.d_ff_shared;
     const int a = t * k;
-    const float* weights = m.in_weights;
-    const int64_t* ids = m.in_ids;
     int rc;
-    if (m.logits) {
-        float* const wout = m.out_weights ? m.out_weights : (float*)(ws + L.weights);
-        int64_t* const iout = m.out_ids ? m.out_ids : (int64_t*)(ws + L.ids);
-        if ((rc = router_topk_impl(m.logits, t, e, k, m.floor_value, m.renormalize, wout, iout, s))) return rc;
-        weights = wout;
-        ids = iout;
-    } else if (m.out_weights || m.out_ids) {
-        hipLaunchKernelGGL(int8_routing_copy_kernel, dim3((a + 255) / 256 < 1024 ? (a + 255) / 256 : 1024), dim3(256), 0, s, weights, ids,
-                           (int64_t)a, m.out_weights, m.out_ids);
-        if ((rc = check_launch("int8 routing copy"))) return rc;
-    }
-    // the sorted arrays behind dropped assignments are never read: chunks cover kept positions only
-    hipLaunchKernelGGL(int8_plan_kernel, dim3(PLAN8_GRID), dim3(PLAN8_THREADS), (size_t)e * 12, s, ids, a, k, e, (int*)(ws + L.row_of),
+    float* const weights = (float*)(ws + L.weights);
+    int64_t* const ids = (int64_t*)(ws + L.ids);
+    const int64_t dp = int8_cols256(d), fp = int8_cols256(f);
+    const int fast = (uintptr_t)m.hidden % 16 == 0 && d % 8 == 0;
+#define QMOE_INT8_ROUTE(DT)                                                                                                            \
+    hipLaunchKernelGGL(int8_route_kernel<DT>, dim3(t), dim3(320), 0, s, m.hidden, d, fast, m.logits, e, k, m.floor_value, m.renormalize, \
+                       m.in_weights, m.in_ids, weights, ids, m.out_weights, m.out_ids, (uint8_t*)(ws + L.q), dp, (float*)(ws + L.s))
+    if (m.hidden_dtype == QMOE_DT_F32) QMOE_INT8_ROUTE(QMOE_DT_F32);
+    else if (m.hidden_dtype == QMOE_DT_F16) QMOE_INT8_ROUTE(QMOE_DT_F16);
+    else QMOE_INT8_ROUTE(QMOE_DT_BF16);
+#undef QMOE_INT8_ROUTE
+    if ((rc = check_launch("int8 expert step (routing)"))) return rc;
+    const int rows = int8_plan_rows(a, e);
+    hipLaunchKernelGGL(int8_plan_kernel, dim3(1), dim3(PLAN8_THREADS), (size_t)e * 8, s, ids, a, k, e, rows, (int*)(ws + L.row_of),
                        (int*)(ws + L.pos_of), (int*)(ws + L.chunk_expert), (int*)(ws + L.chunk_start), (int*)(ws + L.chunk_count),
                        (int*)(ws + L.n_chunks), m.status_out);
-    if ((rc = check_launch("int8 plan"))) return rc;
-    const int64_t dp = int8_cols256(d), fp = int8_cols256(f);
-    if ((rc = int8_quantize_launch(m.hidden, m.hidden_dtype, t, d, (uint8_t*)(ws + L.q), dp, true, (float*)(ws + L.s), s))) return rc;
+    if ((rc = check_launch("int8 expert step (plan)"))) return rc;
+    const int max_chunks = (int)(a / rows + (a < e ? a : e));
     Int8Product p{};
     p.w = (const uint8_t*)m.gate; p.w2 = (const uint8_t*)m.up; p.c = m.gate_scales; p.c2 = m.up_scales;
     p.n = f; p.kp = (int)int8_cols64(d); p.w_step = int8_matrix_bytes(f, d);
@@ -224,25 +287,25 @@ static int int8_moe_impl(const qmoe_int8_moe_args& m, char* ws, const Int8MoeLay
     p.chunk_expert = (const int*)(ws + L.chunk_expert); p.chunk_start = (const int*)(ws + L.chunk_start);
     p.chunk_count = (const int*)(ws + L.chunk_count); p.n_chunks = (const int*)(ws + L.n_chunks);
     p.row_of = (const int*)(ws + L.row_of);
-    if ((rc = int8_product_launch(p, true, L.max_chunks, s))) return rc;
+    if ((rc = int8_plan_launch(p, true, rows, max_chunks, s))) return rc;
     if ((rc = int8_quantize_launch(ws + L.h, QMOE_DT_F32, a, f, (uint8_t*)(ws + L.hq), fp, true, (float*)(ws + L.hs), s))) return rc;
     Int8Product q = p;
     q.w = (const uint8_t*)m.down; q.c = m.down_scales; q.n = d; q.kp = (int)int8_cols64(f); q.w_step = int8_matrix_bytes(d, f);
     q.q = (const uint8_t*)(ws + L.hq); q.ld = fp; q.s = (const float*)(ws + L.hs); q.y = ws + L.terms; q.ldy = d; q.hidden = 0;
     q.row_of = nullptr;
-    if ((rc = int8_product_launch(q, false, L.max_chunks, s))) return rc;
+    if ((rc = int8_plan_launch(q, false, rows, max_chunks, s))) return rc;
     if (fs) {
         const int64_t fsp = int8_cols256(fs);
         Int8Product g{};
         g.w = (const uint8_t*)m.shared_gate_w; g.w2 = (const uint8_t*)m.shared_up_w; g.c = m.shared_gate_scales; g.c2 = m.shared_up_scales;
         g.n = fs; g.kp = p.kp; g.q = p.q; g.ld = dp; g.s = p.s; g.tokens = t; g.y = ws + L.sh; g.ydt = QMOE_DT_F32; g.ldy = fs; g.hidden = 1;
-        if ((rc = int8_product_launch(g, true, 0, s))) return rc;
+        if ((rc = int8_gemm_launch(g, true, s))) return rc;
         if ((rc = int8_quantize_launch(ws + L.sh, QMOE_DT_F32, t, fs, (uint8_t*)(ws + L.shq), fsp, true, (float*)(ws + L.shs), s))) return rc;
         Int8Product o{};
         o.w = (const uint8_t*)m.shared_down_w; o.c = m.shared_down_scales; o.n = d; o.kp = (int)int8_cols64(fs);
         o.q = (const uint8_t*)(ws + L.shq); o.ld = fsp; o.s = (const float*)(ws + L.shs); o.tokens = t; o.y = ws + L.shared_out;
         o.ydt = QMOE_DT_F32; o.ldy = d;
-        if ((rc = int8_product_launch(o, false, 0, s))) return rc;
+        if ((rc = int8_gemm_launch(o, false, s))) return rc;
     }
 #define QMOE_INT8_COMBINE(DT)                                                                                                       \
     hipLaunchKernelGGL(int8_combine_kernel<DT>, dim3(t), dim3(256), 0, s, (const float*)(ws + L.terms), (const int*)(ws + L.pos_of), \
