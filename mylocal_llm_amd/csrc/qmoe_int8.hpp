@@ -138,7 +138,7 @@ struct Int8Product;
 int int8_few_launch(const Int8Product& p, bool pair, const void* x, int xdt, int k, hipStream_t s);
 int int8_gemm_launch(const Int8Product& a, bool pair, hipStream_t s);
 int int8_plan_rows(int64_t assignments, int n_experts);
-int int8_plan_launch(const Int8Product& a, bool pair, int rows, int max_chunks, hipStream_t s);
+int int8_plan_launch(const Int8Product& a, bool pair, int rows, int max_chunks, const Int8Product* side, hipStream_t s);
 
 // One product or one gate/up pair; dense, or over the chunks of a plan (experts' own rows).
 struct Int8Product {

@@ -13,7 +13,8 @@
 namespace qmoe {
 
 template <bool PAIR, bool HIDDEN, bool PLAN, int WN, int WT, int RT, int TT, int KC, int R>
-__global__ __launch_bounds__(64 * WN * WT) void int8_gemm_kernel(const Int8Product a, int n_blocks, int t_blocks) {
+__global__ __launch_bounds__(64 * WN * WT) void int8_gemm_kernel(const Int8Product main_args, int n_blocks, int t_blocks,
+                                                                 const Int8Product side_args, int side_n, int side_t) {
     constexpr int THREADS = 64 * WN * WT, NP = PAIR ? 2 : 1, NW = RT * NP;
     constexpr int ROWS = 16 * TT * WT, PIECES = KC / 16, KK = KC / 64, LOADS = ROWS * PIECES / THREADS;
     // (four pieces a row: two rows are written by eight neighbouring lanes)
@@ -25,12 +26,17 @@ __global__ __launch_bounds__(64 * WN * WT) void int8_gemm_kernel(const Int8Produ
     const int wn = wave % WN, wt = wave / WN, col = lane & 15, g = lane >> 4;
 
     // workgroups go round the eight XCDs: each XCD takes a run of neighbours in the order below, for its L2
-    const int total = PLAN ? n_blocks * *(const QMOE_GLOBAL int*)a.n_chunks : n_blocks * t_blocks;
-    if (PLAN && (int)blockIdx.x >= total) return;
-    const int xcd = blockIdx.x % 8, share = total / 8, over = total % 8;
-    const int id = xcd * share + (xcd < over ? xcd : over) + blockIdx.x / 8;
+    // (a launch over a plan may carry a dense product of the same kind, the shared expert's, in front)
+    const bool aside = PLAN && (int)blockIdx.x < side_n * side_t;
+    const Int8Product a = aside ? side_args : main_args;
+    const int raw = PLAN && !aside ? (int)blockIdx.x - side_n * side_t : (int)blockIdx.x;
+    const int nb = aside ? side_n : n_blocks;
+    const int total = aside ? side_n * side_t : PLAN ? n_blocks * *(const QMOE_GLOBAL int*)a.n_chunks : n_blocks * t_blocks;
+    if (PLAN && raw >= total) return;
+    const int xcd = raw % 8, share = total / 8, over = total % 8;
+    const int id = xcd * share + (xcd < over ? xcd : over) + raw / 8;
     int bn, bt;
-    if (PLAN) { bn = id % n_blocks; bt = id / n_blocks; }
+    if (PLAN) { bn = id % nb; bt = id / nb; }
     else {
         // bands of up to eight token blocks, channel blocks one after the other inside a band
         const int band = id / (8 * n_blocks), in = id % (8 * n_blocks), left = t_blocks - band * 8, high = left < 8 ? left : 8;
@@ -38,7 +44,7 @@ __global__ __launch_bounds__(64 * WN * WT) void int8_gemm_kernel(const Int8Produ
         bn = in / high;
     }
     int first = bt * ROWS, count = a.tokens - first, expert = 0;
-    if (PLAN) {
+    if (PLAN && !aside) {
         expert = a.chunk_expert[bt];
         first = a.chunk_start[bt];
         count = a.chunk_count[bt];
@@ -218,10 +224,13 @@ __global__ __launch_bounds__(64 * WN * WT) void int8_gemm_kernel(const Int8Produ
 }
 
 template <bool PAIR, bool HIDDEN, bool PLAN, int WN, int WT, int RT, int TT, int KC, int R>
-static int gemm8_as(const Int8Product& a, int chunks, hipStream_t s) {
+static int gemm8_as(const Int8Product& a, int chunks, hipStream_t s, const Int8Product* side = nullptr) {
     const int nb = (a.n + 16 * WN * RT - 1) / (16 * WN * RT), tb = PLAN ? chunks : (a.tokens + 16 * WT * TT - 1) / (16 * WT * TT);
-    if ((int64_t)nb * tb > INT32_MAX) return fail(QMOE_EUNSUPPORTED, "int8 product: %d x %d blocks exceed a launch; split the tokens", nb, tb);
-    hipLaunchKernelGGL((int8_gemm_kernel<PAIR, HIDDEN, PLAN, WN, WT, RT, TT, KC, R>), dim3(nb * tb), dim3(64 * WN * WT), 0, s, a, nb, tb);
+    const int sn = side ? (side->n + 16 * WN * RT - 1) / (16 * WN * RT) : 0, st = side ? (side->tokens + 16 * WT * TT - 1) / (16 * WT * TT) : 0;
+    if ((int64_t)nb * tb + (int64_t)sn * st > INT32_MAX)
+        return fail(QMOE_EUNSUPPORTED, "int8 product: %d x %d blocks exceed a launch; split the tokens", nb, tb);
+    hipLaunchKernelGGL((int8_gemm_kernel<PAIR, HIDDEN, PLAN, WN, WT, RT, TT, KC, R>), dim3(nb * tb + sn * st), dim3(64 * WN * WT), 0, s, a, nb, tb,
+                       side ? *side : a, sn, st);
     return check_launch("int8 product");
 }
 
@@ -230,15 +239,16 @@ int int8_plan_rows(int64_t assignments, int n_experts) {
     const int64_t average = assignments / n_experts;
     return average <= 24 ? 32 : average <= 96 ? 64 : 128;
 }
-int int8_plan_launch(const Int8Product& a, bool pair, int rows, int max_chunks, hipStream_t s) {
+// side: NULL, or a dense product of the same kind (pair with the hidden activation, or plain) that rides in front.
+int int8_plan_launch(const Int8Product& a, bool pair, int rows, int max_chunks, const Int8Product* side, hipStream_t s) {
     if (pair) {
-        if (rows == 32) return gemm8_as<true, true, true, 4, 1, 1, 2, 256, 8>(a, max_chunks, s);
-        if (rows == 64) return gemm8_as<true, true, true, 4, 1, 1, 4, 256, 8>(a, max_chunks, s);
-        return gemm8_as<true, true, true, 4, 1, 2, 8, 128, 4>(a, max_chunks, s);
+        if (rows == 32) return gemm8_as<true, true, true, 4, 1, 1, 2, 256, 8>(a, max_chunks, s, side);
+        if (rows == 64) return gemm8_as<true, true, true, 4, 1, 1, 4, 256, 8>(a, max_chunks, s, side);
+        return gemm8_as<true, true, true, 4, 1, 2, 8, 128, 4>(a, max_chunks, s, side);
     }
-    if (rows == 32) return gemm8_as<false, false, true, 4, 1, 2, 2, 256, 8>(a, max_chunks, s);
-    if (rows == 64) return gemm8_as<false, false, true, 4, 1, 2, 4, 256, 8>(a, max_chunks, s);
-    return gemm8_as<false, false, true, 4, 1, 4, 8, 128, 4>(a, max_chunks, s);
+    if (rows == 32) return gemm8_as<false, false, true, 4, 1, 2, 2, 256, 4>(a, max_chunks, s, side);
+    if (rows == 64) return gemm8_as<false, false, true, 4, 1, 2, 4, 256, 8>(a, max_chunks, s, side);
+    return gemm8_as<false, false, true, 4, 1, 4, 8, 128, 4>(a, max_chunks, s, side);
 }
 
 // The largest tile that still gives nearly every CU a workgroup (us; 256 x 256 of eight waves / 256 channels x 64 tokens /
@@ -249,10 +259,6 @@ int int8_gemm_launch(const Int8Product& a, bool pair, hipStream_t s) {
         return (int64_t)((a.n + channels - 1) / channels) * ((a.tokens + tokens - 1) / tokens);
     };
     static constexpr int ENOUGH = 224;
-    if (pair && a.hidden) {
-        if (blocks(128, 64) >= ENOUGH) return gemm8_as<true, true, false, 4, 1, 2, 4, 128, 4>(a, 0, s);
-        return gemm8_as<true, true, false, 4, 1, 1, 2, 256, 8>(a, 0, s);
-    }
     if (pair) {
         if (blocks(128, 256) >= ENOUGH) return gemm8_as<true, false, false, 4, 2, 2, 8, 128, 4>(a, 0, s);
         if (blocks(128, 64) >= ENOUGH) return gemm8_as<true, false, false, 4, 1, 2, 4, 128, 4>(a, 0, s);

@@ -17,7 +17,7 @@ static constexpr int PLAN8_THREADS = 1024;
 static constexpr int PLAN8_MIN_ROWS = 32;     // of a chunk (the workspace is laid out for the most chunks there can be)
 
 // ---- routing and codes of a prompt: a workgroup a token, its first wave routes ---------------------------------
-template <int XDT>
+template <int XDT, int NV>
 __global__ __launch_bounds__(320) void int8_route_kernel(const void* __restrict__ x, int d, int fast, const float* __restrict__ logits,
                                                          int n_experts, int k, float floor_value, int renorm,
                                                          const float* __restrict__ in_weights, const int64_t* __restrict__ in_ids,
@@ -32,7 +32,7 @@ __global__ __launch_bounds__(320) void int8_route_kernel(const void* __restrict_
     if (tid < 0) {
         float w = 0.0f;
         int64_t id = 0;
-        if (logits) router_row<64>(logits + t * n_experts, n_experts, k, floor_value, renorm, w, id, [] {});
+        if (logits) router_row<NV>(logits + t * n_experts, n_experts, k, floor_value, renorm, w, id, [] {});
         else if (lane < k) {
             w = ldg<float>(in_weights + t * k + lane);
             id = ldg<int64_t>(in_ids + t * k + lane);
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(320) void int8_route_kernel(const void* __restrict_
 // products do not depend on its neighbours.  An assignment counts if its id lies in the bank and no earlier slot of its token
 // names it; the others get the position -1 and are reported.
 __global__ __launch_bounds__(PLAN8_THREADS) void int8_plan_kernel(const int64_t* __restrict__ ids, int assignments, int k, int n_experts,
-                                                                  int rows, int* __restrict__ row_of, int* __restrict__ pos_of,
+                                                                  int rows, int check, int* __restrict__ row_of, int* __restrict__ pos_of,
                                                                   int* __restrict__ chunk_expert, int* __restrict__ chunk_start,
                                                                   int* __restrict__ chunk_count, int* __restrict__ n_chunks,
                                                                   int* __restrict__ status_out) {
@@ -93,11 +93,13 @@ __global__ __launch_bounds__(PLAN8_THREADS) void int8_plan_kernel(const int64_t*
     int bad = 0;
     for (int a = tid; a < assignments; a += PLAN8_THREADS) {
         const int64_t e = ldg<int64_t>(ids + a);
-        const int first = a / k * k;
-        int fault = e < 0 || e >= n_experts ? 1 : 0;
-        for (int j = first; j < a; ++j) fault |= ldg<int64_t>(ids + j) == e ? 2 : 0;
-        if (fault & 1) fault = 1;
-        bad |= fault;
+        int fault = 0;
+        if (check) {                             // (the router's own ids are in the bank and no token has one twice)
+            fault = e < 0 || e >= n_experts ? 1 : 0;
+            for (int j = a / k * k; j < a; ++j) fault |= ldg<int64_t>(ids + j) == e ? 2 : 0;
+            if (fault & 1) fault = 1;
+            bad |= fault;
+        }
         pos_of[a] = fault ? -1 : atomicAdd(&count[e], 1);      // (the rank; its expert's start is added below)
     }
     if (bad && status_out) atomicOr(status_out, bad);
@@ -133,6 +135,44 @@ __global__ __launch_bounds__(PLAN8_THREADS) void int8_plan_kernel(const int64_t*
         const int p = start[ldg<int64_t>(ids + a)] + rank;
         pos_of[a] = p;
         row_of[p] = a / k;
+    }
+}
+
+// ---- hidden activations -> codes, the routed rows and the shared expert's in one launch, a workgroup a row ------------
+struct Int8Rows { const float* x; int wide; int64_t ld; uint8_t* codes; float* scales; };
+__global__ __launch_bounds__(256) void int8_hidden_rows_kernel(const Int8Rows routed, int routed_rows, const Int8Rows shared) {
+    __shared__ uint32_t tops[4];
+    const bool sh = (int)blockIdx.x >= routed_rows;
+    const Int8Rows& a = sh ? shared : routed;
+    const int64_t r = sh ? (int)blockIdx.x - routed_rows : (int)blockIdx.x;
+    const float* const x = a.x + r * a.wide;
+    const int tid = threadIdx.x, wide = a.wide;
+    const bool fast = wide % 8 == 0;
+    float v[8];
+    uint32_t top = 0;
+    for (int i0 = 0; i0 < wide; i0 += 2048) {           // (the first 2048 values stay in registers)
+        const int i = i0 + tid * 8;
+        float u[8];
+        int8_load8<QMOE_DT_F32>(x, i < wide ? i : 0, wide - i, fast, u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t b = abs_bits(u[j]);
+            top = b > top ? b : top;
+            if (!i0) v[j] = u[j];
+        }
+    }
+    top = wave_top(top);
+    if ((tid & 63) == 0) tops[tid >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = tops[i] > top ? tops[i] : top;
+    const RowScale rs(top);
+    if (tid == 0) stg<float>(a.scales + r, rs.s);
+    for (int i0 = 0; i0 < a.ld; i0 += 2048) {
+        const int i = i0 + tid * 8;
+        if (i0) int8_load8<QMOE_DT_F32>(x, i < wide ? i : 0, wide - i, fast, v);
+        const u32x2_t q = int8_code8(v, rs);
+        if (i < a.ld) *(QMOE_GLOBAL u32x2_t*)(a.codes + r * a.ld + i) = q;
     }
 }
 
@@ -266,15 +306,16 @@ static int int8_moe_impl(const qmoe_int8_moe_args& m, char* ws, const Int8MoeLay
     const int64_t dp = int8_cols256(d), fp = int8_cols256(f);
     const int fast = (uintptr_t)m.hidden % 16 == 0 && d % 8 == 0;
 #define QMOE_INT8_ROUTE(DT)                                                                                                            \
-    hipLaunchKernelGGL(int8_route_kernel<DT>, dim3(t), dim3(320), 0, s, m.hidden, d, fast, m.logits, e, k, m.floor_value, m.renormalize, \
-                       m.in_weights, m.in_ids, weights, ids, m.out_weights, m.out_ids, (uint8_t*)(ws + L.q), dp, (float*)(ws + L.s))
+    hipLaunchKernelGGL((e <= 1024 ? int8_route_kernel<DT, 16> : int8_route_kernel<DT, 64>), dim3(t), dim3(320), 0, s, m.hidden, d, fast, \
+                       m.logits, e, k, m.floor_value, m.renormalize, m.in_weights, m.in_ids, weights, ids, m.out_weights, m.out_ids,     \
+                       (uint8_t*)(ws + L.q), dp, (float*)(ws + L.s))
     if (m.hidden_dtype == QMOE_DT_F32) QMOE_INT8_ROUTE(QMOE_DT_F32);
     else if (m.hidden_dtype == QMOE_DT_F16) QMOE_INT8_ROUTE(QMOE_DT_F16);
     else QMOE_INT8_ROUTE(QMOE_DT_BF16);
 #undef QMOE_INT8_ROUTE
     if ((rc = check_launch("int8 expert step (routing)"))) return rc;
     const int rows = int8_plan_rows(a, e);
-    hipLaunchKernelGGL(int8_plan_kernel, dim3(1), dim3(PLAN8_THREADS), (size_t)e * 8, s, ids, a, k, e, rows, (int*)(ws + L.row_of),
+    hipLaunchKernelGGL(int8_plan_kernel, dim3(1), dim3(PLAN8_THREADS), (size_t)e * 8, s, ids, a, k, e, rows, m.logits ? 0 : 1, (int*)(ws + L.row_of),
                        (int*)(ws + L.pos_of), (int*)(ws + L.chunk_expert), (int*)(ws + L.chunk_start), (int*)(ws + L.chunk_count),
                        (int*)(ws + L.n_chunks), m.status_out);
     if ((rc = check_launch("int8 expert step (plan)"))) return rc;
@@ -287,26 +328,28 @@ static int int8_moe_impl(const qmoe_int8_moe_args& m, char* ws, const Int8MoeLay
     p.chunk_expert = (const int*)(ws + L.chunk_expert); p.chunk_start = (const int*)(ws + L.chunk_start);
     p.chunk_count = (const int*)(ws + L.chunk_count); p.n_chunks = (const int*)(ws + L.n_chunks);
     p.row_of = (const int*)(ws + L.row_of);
-    if ((rc = int8_plan_launch(p, true, rows, max_chunks, s))) return rc;
-    if ((rc = int8_quantize_launch(ws + L.h, QMOE_DT_F32, a, f, (uint8_t*)(ws + L.hq), fp, true, (float*)(ws + L.hs), s))) return rc;
+    const int64_t fsp = int8_cols256(fs);
+    Int8Product g{};
+    if (fs) {
+        g.w = (const uint8_t*)m.shared_gate_w; g.w2 = (const uint8_t*)m.shared_up_w; g.c = m.shared_gate_scales; g.c2 = m.shared_up_scales;
+        g.n = fs; g.kp = p.kp; g.q = p.q; g.ld = dp; g.s = p.s; g.tokens = t; g.y = ws + L.sh; g.ydt = QMOE_DT_F32; g.ldy = fs; g.hidden = 1;
+    }
+    if ((rc = int8_plan_launch(p, true, rows, max_chunks, fs ? &g : nullptr, s))) return rc;
+    const Int8Rows routed{(const float*)(ws + L.h), f, fp, (uint8_t*)(ws + L.hq), (float*)(ws + L.hs)};
+    const Int8Rows shared{(const float*)(ws + L.sh), fs, fsp, (uint8_t*)(ws + L.shq), (float*)(ws + L.shs)};
+    hipLaunchKernelGGL(int8_hidden_rows_kernel, dim3(a + (fs ? t : 0)), dim3(256), 0, s, routed, a, shared);
+    if ((rc = check_launch("int8 expert step (codes)"))) return rc;
     Int8Product q = p;
     q.w = (const uint8_t*)m.down; q.c = m.down_scales; q.n = d; q.kp = (int)int8_cols64(f); q.w_step = int8_matrix_bytes(d, f);
     q.q = (const uint8_t*)(ws + L.hq); q.ld = fp; q.s = (const float*)(ws + L.hs); q.y = ws + L.terms; q.ldy = d; q.hidden = 0;
     q.row_of = nullptr;
-    if ((rc = int8_plan_launch(q, false, rows, max_chunks, s))) return rc;
+    Int8Product o{};
     if (fs) {
-        const int64_t fsp = int8_cols256(fs);
-        Int8Product g{};
-        g.w = (const uint8_t*)m.shared_gate_w; g.w2 = (const uint8_t*)m.shared_up_w; g.c = m.shared_gate_scales; g.c2 = m.shared_up_scales;
-        g.n = fs; g.kp = p.kp; g.q = p.q; g.ld = dp; g.s = p.s; g.tokens = t; g.y = ws + L.sh; g.ydt = QMOE_DT_F32; g.ldy = fs; g.hidden = 1;
-        if ((rc = int8_gemm_launch(g, true, s))) return rc;
-        if ((rc = int8_quantize_launch(ws + L.sh, QMOE_DT_F32, t, fs, (uint8_t*)(ws + L.shq), fsp, true, (float*)(ws + L.shs), s))) return rc;
-        Int8Product o{};
         o.w = (const uint8_t*)m.shared_down_w; o.c = m.shared_down_scales; o.n = d; o.kp = (int)int8_cols64(fs);
         o.q = (const uint8_t*)(ws + L.shq); o.ld = fsp; o.s = (const float*)(ws + L.shs); o.tokens = t; o.y = ws + L.shared_out;
         o.ydt = QMOE_DT_F32; o.ldy = d;
-        if ((rc = int8_gemm_launch(o, false, s))) return rc;
     }
+    if ((rc = int8_plan_launch(q, false, rows, max_chunks, fs ? &o : nullptr, s))) return rc;
 #define QMOE_INT8_COMBINE(DT)                                                                                                       \
     hipLaunchKernelGGL(int8_combine_kernel<DT>, dim3(t), dim3(256), 0, s, (const float*)(ws + L.terms), (const int*)(ws + L.pos_of), \
                        weights, k, d, fs ? (const float*)(ws + L.shared_out) : nullptr, m.shared_gate, m.hidden, m.residual, m.out,  \
