@@ -113,19 +113,26 @@ __global__ __launch_bounds__(256) void int8_restep_kernel(const uint8_t* __restr
 }
 
 // ---- weight tiles ----------------------------------------------------------------------------------------
-__global__ __launch_bounds__(256) void int8_tiles_kernel(const uint8_t* __restrict__ codes, int64_t n, int64_t k, int64_t pieces,
-                                                         uint8_t* __restrict__ tiles) {
-    const int64_t kt = (k + 63) / 64;
-    for (int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x; p < pieces; p += (int64_t)gridDim.x * 256) {
-        const int lane = (int)(p & 63);
-        const int64_t tile = p >> 6, row = tile / kt * 16 + (lane & 15), col = tile % kt * 64 + (lane >> 4) * 16;
+// A workgroup a row of tiles: 16 rows of codes.  Every row of tiles of all matrices, one behind the other.
+__global__ __launch_bounds__(256) void int8_tiles_kernel(const uint8_t* __restrict__ all_codes, int n, int k, int row_tiles,
+                                                         uint8_t* __restrict__ all_tiles) {
+    const int64_t matrix = blockIdx.x / row_tiles;
+    const int rt = (int)(blockIdx.x % row_tiles), kt = (k + 63) / 64;
+    const uint8_t* const codes = all_codes + matrix * n * (int64_t)k;
+    uint8_t* const tiles = all_tiles + (int64_t)blockIdx.x * kt * 1024;
+    for (int p = threadIdx.x; p < kt * 64; p += 256) {
+        const int lane = p & 63, row = rt * 16 + (lane & 15), col = (p >> 6) * 64 + (lane >> 4) * 16;
         uint32_t v[4] = {0, 0, 0, 0};
-        if (row < n) {
+        if (row < n && col + 16 <= k) {
+            const i32x4_t w = *(const QMOE_GLOBAL i32x4_unaligned_t*)(codes + (int64_t)row * k + col);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = (uint32_t)w[j];
+        } else if (row < n) {
 #pragma unroll
             for (int j = 0; j < 16; ++j)
-                if (col + j < k) v[j >> 2] |= (uint32_t)ldg<uint8_t>(codes + row * k + col + j) << (8 * (j & 3));
+                if (col + j < k) v[j >> 2] |= (uint32_t)ldg<uint8_t>(codes + (int64_t)row * k + col + j) << (8 * (j & 3));
         }
-        *(QMOE_GLOBAL u32x4_t*)(tiles + p * 16) = u32x4_t{v[0], v[1], v[2], v[3]};
+        *(QMOE_GLOBAL u32x4_t*)(tiles + (int64_t)p * 16) = u32x4_t{v[0], v[1], v[2], v[3]};
     }
 }
 
@@ -154,20 +161,20 @@ static int dense(const char* who, bool pair, const void* w, const float* c, cons
     a.n = n; a.kp = (int)int8_cols64(k); a.tokens = tokens; a.y = y; a.ydt = ydt; a.ldy = n; a.ld = int8_cols256(k);
     a.q = (const uint8_t*)x; a.s = xs;
     if (xdt != QMOE_DT_I8 && int8_few_fuses(tokens, k)) return int8_few_launch(a, pair, x, xdt, k, st);
-    if (!direct) {
-        uint8_t* q = (uint8_t*)workspace;
+    const bool few = int8_few_takes(n, tokens);
+    if (xdt != QMOE_DT_I8) {
+        uint8_t* const q = (uint8_t*)workspace;
+        float* const s = (float*)(q + round256((size_t)tokens * a.ld));
         a.q = q;
-        if (xdt == QMOE_DT_I8) {
-            hipLaunchKernelGGL(int8_restep_kernel, dim3(tokens), dim3(256), 0, st, (const uint8_t*)x, k, q, a.ld);
-            if (const int rc = check_launch(who)) return rc;
-        } else {
-            float* s = (float*)(q + round256((size_t)tokens * a.ld));
-            a.s = s;
-            if (const int rc = int8_quantize_launch(x, xdt, tokens, k, q, a.ld, true, s, st)) return rc;
-        }
+        a.s = s;
+        if (const int rc = int8_quantize_launch(x, xdt, tokens, k, q, a.ld, true, s, st)) return rc;
+    } else if (few) a.ld = k;            // (read as they are, at any alignment)
+    else if (!direct) {
+        a.q = (const uint8_t*)workspace;
+        hipLaunchKernelGGL(int8_restep_kernel, dim3(tokens), dim3(256), 0, st, (const uint8_t*)x, k, (uint8_t*)workspace, a.ld);
+        if (const int rc = check_launch(who)) return rc;
     }
-    if (tokens <= INT8_FEW_TOKENS) return int8_few_launch(a, pair, nullptr, 0, k, st);
-    return int8_gemm_launch(a, pair, st);
+    return few ? int8_few_launch(a, pair, nullptr, 0, k, st) : int8_gemm_launch(a, pair, st);
 }
 
 }  // namespace qmoe
@@ -195,17 +202,16 @@ int qmoe_int8_tiles(const void* codes, int64_t matrices, int n, int k, void* til
     if (matrices < 1 || n < 1 || k < 1) return fail(QMOE_EINVAL, "%s: matrices=%lld n=%d k=%d", who, (long long)matrices, n, k);
     if (k > INT8_MAX_K) return fail(QMOE_EUNSUPPORTED, "%s: K=%d beyond %d, where an int32 sum could overflow", who, k, INT8_MAX_K);
     if ((uintptr_t)tiles % 16) return fail(QMOE_EINVAL, "%s: tiles must be 16-byte aligned", who);
-    const int64_t pieces = int8_matrix_bytes(n, k) / 16;
-    const int64_t blocks = (pieces + 255) / 256;
-    for (int64_t m = 0; m < matrices; ++m)
-        hipLaunchKernelGGL(int8_tiles_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, (hipStream_t)stream,
-                           (const uint8_t*)codes + m * n * (int64_t)k, (int64_t)n, (int64_t)k, pieces, (uint8_t*)tiles + m * pieces * 16);
+    const int row_tiles = (int)(int8_rows16(n) / 16);
+    if (matrices * row_tiles > INT32_MAX) return fail(QMOE_EUNSUPPORTED, "%s: more than 2^31 - 1 rows of tiles; lay the matrices out in parts", who);
+    hipLaunchKernelGGL(int8_tiles_kernel, dim3((unsigned)(matrices * row_tiles)), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)codes, n, k,
+                       row_tiles, (uint8_t*)tiles);
     return check_launch(who);
 }
 
 size_t qmoe_int8_workspace_bytes(int n, int k, int tokens, int x_dtype) {
     if (n < 1 || k < 1 || tokens < 1) return 0;
-    if (x_dtype != QMOE_DT_INT8 && int8_few_fuses(tokens, k)) return 0;
+    if (x_dtype == QMOE_DT_INT8 ? int8_few_takes(n, tokens) : int8_few_fuses(tokens, k)) return 0;
     return round256((size_t)tokens * (size_t)int8_cols256(k)) + round256((size_t)tokens * 4);
 }
 

@@ -17,6 +17,8 @@
 namespace qmoe {
 
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef i32x4_t i32x4_unaligned_t __attribute__((aligned(1)));      // (one request all the same)
+typedef i32x4_t i32x4_dword_t __attribute__((aligned(4)));
 
 static constexpr int INT8_MAX_K = 131071;     // 128 * 128 * K stays inside int32
 static constexpr int QMOE_DT_I8 = QMOE_DT_INT8;
@@ -130,10 +132,10 @@ __device__ __forceinline__ void meet_lds() {
 // x rows -> codes (row step ld bytes; pad: zeros up to the next multiple of 256 columns) + scales
 int int8_quantize_launch(const void* x, int dt, int64_t rows, int k, uint8_t* codes, int64_t ld, bool pad, float* scales, hipStream_t s);
 
-static constexpr int INT8_FEW_TOKENS = 64;
-// Whether a product of these rows quantises them in its own workgroups, and the launch for up to 64 tokens (x: rows to
-// quantise, NULL: p.q holds codes).
+// Whether a product of these rows quantises them in its own workgroups, whether it is one of few tokens, and its launch (x: rows
+// to quantise, NULL: p.q holds codes, any alignment).
 bool int8_few_fuses(int tokens, int k);
+bool int8_few_takes(int n, int tokens);
 struct Int8Product;
 int int8_few_launch(const Int8Product& p, bool pair, const void* x, int xdt, int k, hipStream_t s);
 int int8_gemm_launch(const Int8Product& a, bool pair, hipStream_t s);

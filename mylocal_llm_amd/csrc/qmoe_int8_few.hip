@@ -17,8 +17,8 @@ struct Few8Args {
     const float *c, *c2;
     int n, kp, steps;       // steps = kp / 64
     const void* x;          // fused: rows to quantise
-    int k, fast;            // columns; rows may be read 16 bytes at a time
-    const uint8_t* q;       // otherwise: codes, their row step and scales
+    int k, fast;            // columns; rows of x may be read 16 bytes at a time
+    const uint8_t* q;       // otherwise: codes, their row step and scales (any alignment; k of them may be read in a row)
     int64_t ld;
     const float* s;
     int tokens;
@@ -26,13 +26,13 @@ struct Few8Args {
     int ydt;
 };
 
-// NX > 0: every workgroup quantises the rows itself (they are few: up to NX pieces of 4096 columns of a token, eight
+// NX < 0: rows of codes at any address, NX = 0: at multiples of four bytes, NX > 0: every workgroup quantises the rows itself (they are few: up to NX pieces of 4096 columns of a token, eight
 // values a thread and piece, kept in registers between the search for the largest and the codes), into LDS rows
 // kp + 16 bytes apart: eight neighbouring tokens' 16-byte pieces then lie in eight different bank groups.  The rows are
 // requested before the first weights, so that waiting for them does not wait for the weights.
 template <int XDT, bool PAIR, int NX, int TT, int RT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Few8Args a) {
-    constexpr bool FUSED = NX > 0;
+    constexpr bool FUSED = NX > 0, SHIFT = NX < 0;
     constexpr int THREADS = 64 * WAVES;
     constexpr int NP = PAIR ? 2 : 1, NW = RT * NP, U = NW >= 8 ? 1 : 8 / NW;
     extern __shared__ uint8_t lds[];       // [codes] and, over them at the end, [waves][NW][TT][64] partial sums
@@ -41,6 +41,7 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Few8Args a) 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
     const int row_tiles = (a.n + 15) / 16;
+    const int first = FUSED ? 0 : (int)blockIdx.y * 16 * TT, tokens = a.tokens - first < 16 * TT ? a.tokens - first : 16 * TT;
 
     constexpr int PIECE = THREADS * 8;
     const int per = (a.k + PIECE - 1) / PIECE;     // pieces of a token
@@ -48,7 +49,7 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Few8Args a) 
     if (FUSED) {
 #pragma unroll
         for (int p = 0; p < NX; ++p) {
-            const int t = p / per, i = (p % per) * PIECE + tid * 8, left = t < a.tokens ? a.k - i : 0;
+            const int t = p / per, i = (p % per) * PIECE + tid * 8, left = t < tokens ? a.k - i : 0;
             int8_load8<XDT>(a.x, left > 0 ? (size_t)t * a.k + i : 0, left, a.fast, v[p]);
         }
     }
@@ -62,7 +63,9 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Few8Args a) 
         if (PAIR) wp[r * NP + 1] = a.w2 + (int64_t)tile * a.kp * 16 + lane * 16;
     }
     // this wave's steps; one without a step of its own (K below 512) requests its neighbour's and multiplies none
-    const int lo = a.steps * wave / WAVES, hi = a.steps * (wave + 1) / WAVES, last = hi > lo ? hi - 1 : lo < a.steps ? lo : a.steps - 1;
+    // (codes read as they are: a last step that is not whole is left to the end)
+    const int whole = FUSED ? a.steps : a.k / 64, lo = a.steps * wave / WAVES, end = a.steps * (wave + 1) / WAVES, hi = end < whole ? end : whole;
+    const int last = hi > lo ? hi - 1 : lo < a.steps ? lo : a.steps - 1;
     i32x4_t wr[U][NW];
     auto request = [&](int chunk) {
 #pragma unroll
@@ -76,6 +79,9 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Few8Args a) 
 
     const int stride = a.kp + 16;
     const uint8_t* qp[TT];
+    uint32_t shift[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) shift[t] = 0;
     if (FUSED) {
 #pragma unroll
         for (int p = 0; p < NX; ++p) {
@@ -89,7 +95,7 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Few8Args a) 
 #pragma unroll
         for (int p = 0; p < NX; ++p) {
             const int t = p / per, i = (p % per) * PIECE + tid * 8;
-            if (t >= a.tokens) break;
+            if (t >= tokens) break;
             uint32_t top = 0;
             for (int j = t * per * WAVES; j < (t + 1) * per * WAVES; ++j) top = tops[j] > top ? tops[j] : top;
             const RowScale rs(top);
@@ -101,9 +107,10 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Few8Args a) 
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
             const int row = t * 16 + col;
-            qp[t] = a.q + (int64_t)(row < a.tokens ? row : a.tokens - 1) * a.ld + g * 16;
+            qp[t] = a.q + (int64_t)(first + (row < tokens ? row : tokens - 1)) * a.ld + g * 16;
+            if (SHIFT) shift[t] = (uint32_t)(uintptr_t)qp[t] & 3u;
         }
-        if (tid < 16 * TT) srow[tid] = tid < a.tokens ? a.s[tid] : 0.0f;
+        if (tid < 16 * TT) srow[tid] = tid < tokens ? a.s[first + tid] : 0.0f;
     }
 
     i32x4_t acc[NW][TT];
@@ -111,16 +118,38 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Few8Args a) 
     for (int i = 0; i < NW; ++i)
 #pragma unroll
         for (int t = 0; t < TT; ++t) acc[i][t] = i32x4_t{0, 0, 0, 0};
-    const int chunks = (hi - lo + U - 1) / U;
-    const uint8_t* const mine = lds + (col < a.tokens ? col : a.tokens - 1) * stride + g * 16;
+    if (!FUSED && end > hi && end > lo) {      // the row's end: bytes, zeros behind it
+        const int c = whole * 64 + g * 16;
+        i32x4_t w[NW];
+#pragma unroll
+        for (int i = 0; i < NW; ++i) w[i] = ldg_i32x4(wp[i] + (int64_t)whole * 1024);
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+            uint32_t v[16];
+            i32x4_t b;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = ldg<uint8_t>(qp[t] + (c + i < a.k ? c + i : a.k - 1) - g * 16);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = c + i < a.k ? v[i] << (8 * (i & 3)) : 0u;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j] = (int)(v[4 * j] | v[4 * j + 1] | v[4 * j + 2] | v[4 * j + 3]);
+#pragma unroll
+            for (int i = 0; i < NW; ++i) acc[i][t] = mfma_i8(w[i], b, acc[i][t]);
+        }
+    }
+    const int chunks = hi > lo ? (hi - lo + U - 1) / U : 0;
+    const uint8_t* const mine = lds + (col < tokens ? col : tokens - 1) * stride + g * 16;
     for (int chunk = 0; chunk < chunks; ++chunk) {
         i32x4_t now[U][NW], b[U][TT];
+        int next[SHIFT ? U : 1][TT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int step = lo + chunk * U + u < last ? lo + chunk * U + u : last;
+            const int step = lo + chunk * U + u < hi - 1 ? lo + chunk * U + u : hi - 1;
 #pragma unroll
-            for (int t = 0; t < TT; ++t)
-                b[u][t] = FUSED ? *(const i32x4_t*)(mine + step * 64) : ldg_i32x4(qp[t] + (int64_t)step * 64);
+            for (int t = 0; t < TT; ++t) {
+                b[u][t] = FUSED ? *(const i32x4_t*)(mine + step * 64) : *(const QMOE_GLOBAL i32x4_dword_t*)(qp[t] - shift[t] + (int64_t)step * 64);
+                if (SHIFT) next[u][t] = ldg<int>(qp[t] - shift[t] + (int64_t)step * 64 + (shift[t] ? 16 : 12));
+            }
 #pragma unroll
             for (int i = 0; i < NW; ++i) now[u][i] = wr[u][i];
         }
@@ -128,6 +157,14 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Few8Args a) 
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (lo + chunk * U + u < hi) {
+                if (SHIFT) {
+#pragma unroll
+                    for (int t = 0; t < TT; ++t) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            b[u][t][j] = (int)__builtin_amdgcn_alignbyte(j < 3 ? (uint32_t)b[u][t][(j + 1) & 3] : (uint32_t)next[u][t], (uint32_t)b[u][t][j], shift[t]);
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < NW; ++i)
 #pragma unroll
@@ -142,7 +179,7 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Few8Args a) 
         for (int t = 0; t < TT; ++t) *(i32x4_t*)(part + ((size_t)(wave * NW + i) * TT + t) * 256 + lane * 4) = acc[i][t];
     __syncthreads();
     // (token, channel) of this thread: channel fastest; the sum of channel 4 g + i and token c is value i of lane 16 g + c
-    for (int o = tid; o < a.tokens * RT * 16; o += THREADS) {
+    for (int o = tid; o < tokens * RT * 16; o += THREADS) {
         const int ch = o % (RT * 16), t = o / (RT * 16), r = ch >> 4, in = ch & 15;
         const int n = blockIdx.x * RT * 16 + ch;
         if (n >= a.n) continue;
@@ -155,14 +192,14 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Few8Args a) 
         }
         const double v = int8_value(s0, srow[t], a.c[n]);
         const float out = PAIR ? int8_hidden(v, int8_value(s1, srow[t], a.c2[n])) : (float)v;
-        store_out(a.y, a.ydt, (size_t)t * a.n + n, out);
+        store_out(a.y, a.ydt, (size_t)(first + t) * a.n + n, out);
     }
 }
 
 template <int XDT, bool PAIR, int NX, int TT, int RT, int WAVES>
 static int few8_as(const Few8Args& a, hipStream_t s) {
     constexpr int NW = RT * (PAIR ? 2 : 1);
-    const size_t partial = (size_t)WAVES * NW * TT * 1024, codes = NX ? (size_t)a.tokens * (a.kp + 16) : 0;
+    const size_t partial = (size_t)WAVES * NW * TT * 1024, codes = NX > 0 ? (size_t)a.tokens * (a.kp + 16) : 0;
     const size_t lds = partial > codes ? partial : codes;
     const void* fn = (const void*)&int8_few_kernel<XDT, PAIR, NX, TT, RT, WAVES>;
     if (lds > 64 * 1024) {
@@ -175,7 +212,7 @@ static int few8_as(const Few8Args& a, hipStream_t s) {
             if (dev >= 0 && dev < 64) raised[dev] = true;
         }
     }
-    hipLaunchKernelGGL((int8_few_kernel<XDT, PAIR, NX, TT, RT, WAVES>), dim3((a.n + 16 * RT - 1) / (16 * RT)), dim3(64 * WAVES), lds, s, a);
+    hipLaunchKernelGGL((int8_few_kernel<XDT, PAIR, NX, TT, RT, WAVES>), dim3((a.n + 16 * RT - 1) / (16 * RT), NX > 0 ? 1 : (a.tokens + 16 * TT - 1) / (16 * TT)), dim3(64 * WAVES), lds, s, a);
     return check_launch("int8 product of a few tokens");
 }
 
@@ -184,11 +221,17 @@ static int few8_as(const Few8Args& a, hipStream_t s) {
 static int few8_pieces(int k) { return (k + 4095) / 4096; }
 bool int8_few_fuses(int tokens, int k) { return tokens == 1 && few8_pieces(k) <= 4; }
 
+// Up to 64 tokens, and more where 64 x 64 tiles would leave most of the chip without a workgroup.
+bool int8_few_takes(int n, int tokens) { return tokens <= 64 || ((n + 63ll) / 64) * ((tokens + 63ll) / 64) < 96; }
+
 template <int XDT, bool PAIR, int RT> static int few8_fused(const Few8Args& a, int waves, hipStream_t s) {
     if (waves == 16) return few8_pieces(a.k) <= 2 ? few8_as<XDT, PAIR, 1, 1, 1, 16>(a, s) : few8_as<XDT, PAIR, 2, 1, 1, 16>(a, s);
     return few8_pieces(a.k) == 1 ? few8_as<XDT, PAIR, 1, 1, RT, 8>(a, s) : few8_as<XDT, PAIR, 4, 1, RT, 8>(a, s);
 }
 template <bool PAIR> static int few8_codes(const Few8Args& a, int rt, int waves, hipStream_t s) {
+    // rows at odd addresses: whole dwords and a shift (as they are, 77 x 1001 x 1234 takes 10.9 us, so 7.6, at multiples of four 5.4)
+    if (((uintptr_t)a.q | (uintptr_t)a.ld) % 4) return a.tokens <= 16 ? few8_as<0, PAIR, -1, 1, 1, 8>(a, s) : few8_as<0, PAIR, -1, 2, 1, 8>(a, s);
+    if (a.tokens > 64) return few8_as<0, PAIR, 0, 2, 1, 8>(a, s);      // blocks of 32 tokens
     if (a.tokens <= 16) return waves == 16 ? few8_as<0, PAIR, 0, 1, 1, 16>(a, s) : rt == 1 ? few8_as<0, PAIR, 0, 1, 1, 8>(a, s) : few8_as<0, PAIR, 0, 1, 2, 8>(a, s);
     if (a.tokens <= 32) return rt == 1 ? few8_as<0, PAIR, 0, 2, 1, 8>(a, s) : few8_as<0, PAIR, 0, 2, 2, 8>(a, s);
     return rt == 1 ? few8_as<0, PAIR, 0, 4, 1, 8>(a, s) : rt == 2 || PAIR ? few8_as<0, PAIR, 0, 4, 2, 8>(a, s) : few8_as<0, PAIR, 0, 4, PAIR ? 2 : 4, 8>(a, s);
@@ -205,8 +248,9 @@ int int8_few_launch(const Int8Product& p, bool pair, const void* x, int xdt, int
     const int tiles = (p.n + 15) / 16;
     const int rt = tiles < 512 ? 1 : tiles >= 768 && p.tokens > 32 ? 4 : 2;
     const int waves = x && k > 4096 && tiles < 512 ? 16 : 8;
+    a.k = x ? k : (int)(p.ld < p.kp ? k : p.kp);
     if (!x) return pair ? few8_codes<true>(a, rt, waves, s) : few8_codes<false>(a, rt, waves, s);
-    a.x = x; a.k = k;
+    a.x = x;
     a.fast = (uintptr_t)x % 16 == 0 && k % 8 == 0;
 #define QMOE_FUSED(DT) (pair ? few8_fused<DT, true, 1>(a, waves, s) : rt == 1 ? few8_fused<DT, false, 1>(a, waves, s) : few8_fused<DT, false, 2>(a, waves, s))
     if (xdt == QMOE_DT_F32) return QMOE_FUSED(QMOE_DT_F32);

@@ -50,7 +50,8 @@ def test_sizes():
     assert lib.qmoe_int8_matrix_bytes(70000, 65536) == 70000 * 65536
     a, b = lib.qmoe_int8_workspace_bytes(64, 100, 3, 0), lib.qmoe_int8_workspace_bytes(64, 100, 30, 2)
     assert 0 < a < b and a % 256 == b % 256 == 0 and lib.qmoe_int8_workspace_bytes(64, 100, 0, 0) == 0
-    assert lib.qmoe_int8_workspace_bytes(64, 100, 1, 0) == 0 and lib.qmoe_int8_workspace_bytes(64, 100, 1, 3) > 0
+    assert lib.qmoe_int8_workspace_bytes(64, 100, 1, 0) == 0 and lib.qmoe_int8_workspace_bytes(64, 100, 1, 3) == 0
+    assert lib.qmoe_int8_workspace_bytes(20000, 100, 500, 3) > 0
     m = [lib.qmoe_int8_moe_workspace_bytes(t, 10, 512, 2048, 512, 2048) for t in (1, 16, 4096)]
     assert 0 < m[0] < m[1] < m[2] and lib.qmoe_int8_moe_workspace_bytes(1, 0, 4, 4, 4, 0) == 0
 
