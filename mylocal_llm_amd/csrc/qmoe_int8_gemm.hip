@@ -13,7 +13,7 @@
 namespace qmoe {
 
 template <bool PAIR, bool HIDDEN, bool PLAN, int WN, int WT, int RT, int TT, int KC, int R>
-__global__ __launch_bounds__(64 * WN * WT) void int8_gemm_kernel(const Int8Product main_args, int n_blocks, int t_blocks,
+__global__ __launch_bounds__(64 * WN * WT) __attribute__((amdgpu_waves_per_eu(2))) void int8_gemm_kernel(const Int8Product main_args, int n_blocks, int t_blocks,
                                                                  const Int8Product side_args, int side_n, int side_t) {
     constexpr int THREADS = 64 * WN * WT, NP = PAIR ? 2 : 1, NW = RT * NP;
     constexpr int ROWS = 16 * TT * WT, PIECES = KC / 16, KK = KC / 64, LOADS = ROWS * PIECES / THREADS;
@@ -251,22 +251,25 @@ int int8_plan_launch(const Int8Product& a, bool pair, int rows, int max_chunks, 
     return gemm8_as<false, false, true, 4, 1, 4, 8, 128, 4>(a, max_chunks, s, side);
 }
 
-// The largest tile that still gives nearly every CU a workgroup (us; 256 x 256 of eight waves / 256 channels x 64 tokens /
-// 64 x 64, activations quantised on the way): 4096 tokens x 14336 x 4096 298 / 309 / 400, 1024 x 4096 x 4096 70 / 34 / 37,
-// 512 x 14336 x 4096 69 / 48 / 55, 128 x 4096 x 4096 57 / 29 / 15.
+// The largest tile that still gives nearly every CU a workgroup (us from codes; 256 x 256 of eight waves / 256 channels x
+// 128 tokens of four, two workgroups a CU / 256 x 64 / 64 x 64): 4096 tokens x 4096 x 14336 177 / 183 / 250 / 360,
+// 4096 x 14336 x 4096 222 / 208 / 245 / 380, 1024 x 4096 x 4096 58 / 38 / 23 / 35, 128 x 4096 x 4096 42 / - / 27 / 11.
+// One workgroup a CU loses what the last round leaves empty, and nothing hides its start and its end: the largest tile is
+// taken where the rounds come out nearly even.
 int int8_gemm_launch(const Int8Product& a, bool pair, hipStream_t s) {
     auto blocks = [&](int channels, int tokens) {
         return (int64_t)((a.n + channels - 1) / channels) * ((a.tokens + tokens - 1) / tokens);
     };
-    static constexpr int ENOUGH = 224;
-    if (pair) {
-        if (blocks(128, 256) >= ENOUGH) return gemm8_as<true, false, false, 4, 2, 2, 8, 128, 4>(a, 0, s);
-        if (blocks(128, 64) >= ENOUGH) return gemm8_as<true, false, false, 4, 1, 2, 4, 128, 4>(a, 0, s);
-        return gemm8_as<true, false, false, 4, 1, 1, 2, 256, 8>(a, 0, s);
-    }
-    if (blocks(256, 256) >= ENOUGH) return gemm8_as<false, false, false, 4, 2, 4, 8, 128, 4>(a, 0, s);
-    if (blocks(256, 64) >= ENOUGH) return gemm8_as<false, false, false, 4, 1, 4, 4, 128, 4>(a, 0, s);
-    return gemm8_as<false, false, false, 4, 1, 1, 4, 256, 8>(a, 0, s);
+    static constexpr int CUS = 256, ENOUGH = 224;
+    const int wide = pair ? 128 : 256;
+    const int64_t large = blocks(wide, 256), rounds = (large + CUS - 1) / CUS * CUS;
+    if (large >= ENOUGH && large * 20 >= rounds * 19)
+        return pair ? gemm8_as<true, false, false, 4, 2, 2, 8, 128, 4>(a, 0, s) : gemm8_as<false, false, false, 4, 2, 4, 8, 128, 4>(a, 0, s);
+    if (blocks(wide, 128) >= ENOUGH)
+        return pair ? gemm8_as<true, false, false, 4, 1, 2, 8, 128, 4>(a, 0, s) : gemm8_as<false, false, false, 4, 1, 4, 8, 128, 4>(a, 0, s);
+    if (blocks(wide, 64) >= ENOUGH)
+        return pair ? gemm8_as<true, false, false, 4, 1, 2, 4, 128, 4>(a, 0, s) : gemm8_as<false, false, false, 4, 1, 4, 4, 128, 4>(a, 0, s);
+    return pair ? gemm8_as<true, false, false, 4, 1, 1, 2, 256, 8>(a, 0, s) : gemm8_as<false, false, false, 4, 1, 1, 4, 256, 8>(a, 0, s);
 }
 
 }  // namespace qmoe
