@@ -31,13 +31,18 @@ __global__ __launch_bounds__(64 * WN * WT) __attribute__((amdgpu_waves_per_eu(2)
     const Int8Product a = aside ? side_args : main_args;
     const int raw = PLAN && !aside ? (int)blockIdx.x - side_n * side_t : (int)blockIdx.x;
     const int nb = aside ? side_n : n_blocks;
-    const int total = aside ? side_n * side_t : PLAN ? n_blocks * *(const QMOE_GLOBAL int*)a.n_chunks : n_blocks * t_blocks;
-    if (PLAN && raw >= total) return;
+    const int total = aside ? side_n * side_t : n_blocks * t_blocks;
     const int xcd = raw % 8, share = total / 8, over = total % 8;
     const int id = xcd * share + (xcd < over ? xcd : over) + raw / 8;
     int bn, bt;
-    if (PLAN) { bn = id % nb; bt = id / nb; }
-    else {
+    if (aside) { bn = id % nb; bt = id / nb; }
+    else if (PLAN) {
+        // runs of four chunks an XCD, whatever their number turns out to be: it is not waited for to find the chunk
+        const int c = raw / 8 / nb;
+        bn = raw / 8 % nb;
+        bt = c / 4 * 32 + xcd * 4 + c % 4;
+        if (bt >= t_blocks) return;
+    } else {
         // bands of up to eight token blocks, channel blocks one after the other inside a band
         const int band = id / (8 * n_blocks), in = id % (8 * n_blocks), left = t_blocks - band * 8, high = left < 8 ? left : 8;
         bt = band * 8 + in % high;
@@ -48,6 +53,7 @@ __global__ __launch_bounds__(64 * WN * WT) __attribute__((amdgpu_waves_per_eu(2)
         expert = a.chunk_expert[bt];
         first = a.chunk_start[bt];
         count = a.chunk_count[bt];
+        if (bt >= *(const QMOE_GLOBAL int*)a.n_chunks) return;      // (what lies behind the last chunk was loaded, not used)
     }
 
     const int row_tiles = (a.n + 15) / 16, steps = a.kp / 64, chunks = (a.kp + KC - 1) / KC;
@@ -225,11 +231,11 @@ __global__ __launch_bounds__(64 * WN * WT) __attribute__((amdgpu_waves_per_eu(2)
 
 template <bool PAIR, bool HIDDEN, bool PLAN, int WN, int WT, int RT, int TT, int KC, int R>
 static int gemm8_as(const Int8Product& a, int chunks, hipStream_t s, const Int8Product* side = nullptr) {
-    const int nb = (a.n + 16 * WN * RT - 1) / (16 * WN * RT), tb = PLAN ? chunks : (a.tokens + 16 * WT * TT - 1) / (16 * WT * TT);
+    const int nb = (a.n + 16 * WN * RT - 1) / (16 * WN * RT), tb = PLAN ? (chunks + 31) / 32 * 32 : (a.tokens + 16 * WT * TT - 1) / (16 * WT * TT);
     const int sn = side ? (side->n + 16 * WN * RT - 1) / (16 * WN * RT) : 0, st = side ? (side->tokens + 16 * WT * TT - 1) / (16 * WT * TT) : 0;
     if ((int64_t)nb * tb + (int64_t)sn * st > INT32_MAX)
         return fail(QMOE_EUNSUPPORTED, "int8 product: %d x %d blocks exceed a launch; split the tokens", nb, tb);
-    hipLaunchKernelGGL((int8_gemm_kernel<PAIR, HIDDEN, PLAN, WN, WT, RT, TT, KC, R>), dim3(nb * tb + sn * st), dim3(64 * WN * WT), 0, s, a, nb, tb,
+    hipLaunchKernelGGL((int8_gemm_kernel<PAIR, HIDDEN, PLAN, WN, WT, RT, TT, KC, R>), dim3(nb * tb + sn * st), dim3(64 * WN * WT), 0, s, a, nb, PLAN ? chunks : tb,
                        side ? *side : a, sn, st);
     return check_launch("int8 product");
 }
@@ -252,8 +258,9 @@ int int8_plan_launch(const Int8Product& a, bool pair, int rows, int max_chunks, 
 }
 
 // The largest tile that still gives nearly every CU a workgroup (us from codes; 256 x 256 of eight waves / 256 channels x
-// 128 tokens of four, two workgroups a CU / 256 x 64 / 64 x 64): 4096 tokens x 4096 x 14336 177 / 183 / 250 / 360,
-// 4096 x 14336 x 4096 222 / 208 / 245 / 380, 1024 x 4096 x 4096 58 / 38 / 23 / 35, 128 x 4096 x 4096 42 / - / 27 / 11.
+// 128 tokens of four, two workgroups a CU / 256 x 64 / 64 x 64): 4096 tokens x 4096 x 14336 184 / 184 / 220 / 351,
+// 4096 x 14336 x 4096 225 / 213 / 268 / 380, 512 x 14336 x 4096 49 / 33 / 36 / 48, 1024 x 4096 x 4096 47 / 30 / 21 / 30,
+// 128 x 4096 x 4096 42 / 29 / 17 / 10.
 // One workgroup a CU loses what the last round leaves empty, and nothing hides its start and its end: the largest tile is
 // taken where the rounds come out nearly even.
 int int8_gemm_launch(const Int8Product& a, bool pair, hipStream_t s) {

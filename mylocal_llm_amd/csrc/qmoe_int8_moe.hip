@@ -10,7 +10,7 @@
 namespace qmoe {
 
 bool int8_step_covers(int tokens, int k, int n_experts, int d, int f, int fs);
-size_t int8_step_bytes(int tokens, int k, int f, int fs);
+size_t int8_step_bytes(int tokens, int k, int d, int f, int fs);
 int int8_step_launch(const qmoe_int8_moe_args& m, char* ws, hipStream_t s);
 
 static constexpr int PLAN8_THREADS = 1024;
@@ -74,6 +74,21 @@ __global__ __launch_bounds__(320) void int8_route_kernel(const void* __restrict_
     }
 }
 
+// weights / ids of every token (also to the caller's arrays), codes with row step ld (a multiple of 8, the tail zero) + scales
+int int8_route_launch(const qmoe_int8_moe_args& m, float* weights, int64_t* ids, uint8_t* codes, int64_t ld, float* scales, hipStream_t s) {
+    const int t = m.tokens, k = m.top_k, e = m.n_experts, d = m.d_model;
+    const int fast = (uintptr_t)m.hidden % 16 == 0 && d % 8 == 0;
+#define QMOE_INT8_ROUTE(DT)                                                                                                              \
+    hipLaunchKernelGGL((e <= 1024 ? int8_route_kernel<DT, 16> : int8_route_kernel<DT, 64>), dim3(t), dim3(320), 0, s, m.hidden, d, fast, \
+                       m.logits, e, k, m.floor_value, m.renormalize, m.in_weights, m.in_ids, weights, ids, m.out_weights, m.out_ids,     \
+                       codes, ld, scales)
+    if (m.hidden_dtype == QMOE_DT_F32) QMOE_INT8_ROUTE(QMOE_DT_F32);
+    else if (m.hidden_dtype == QMOE_DT_F16) QMOE_INT8_ROUTE(QMOE_DT_F16);
+    else QMOE_INT8_ROUTE(QMOE_DT_BF16);
+#undef QMOE_INT8_ROUTE
+    return check_launch("int8 expert step (routing)");
+}
+
 // ---- plan ------------------------------------------------------------------------------------------------
 // One workgroup groups the assignments by expert.  The place of an assignment inside its expert is the order in which the
 // adds to the expert's counter happened: it may differ from run to run, and no result depends on it, since a row's
@@ -91,8 +106,10 @@ __global__ __launch_bounds__(PLAN8_THREADS) void int8_plan_kernel(const int64_t*
     for (int e = tid; e < n_experts; e += PLAN8_THREADS) count[e] = 0;
     __syncthreads();
     int bad = 0;
-    for (int a = tid; a < assignments; a += PLAN8_THREADS) {
-        const int64_t e = ldg<int64_t>(ids + a);
+    // the expert and the rank of this thread's first assignments stay in registers, the others' ranks lie in pos_of meanwhile
+    constexpr int NR = 8;
+    int mine[NR], rank[NR];
+    auto count_in = [&](int a, int64_t e) -> int {
         int fault = 0;
         if (check) {                             // (the router's own ids are in the bank and no token has one twice)
             fault = e < 0 || e >= n_experts ? 1 : 0;
@@ -100,8 +117,20 @@ __global__ __launch_bounds__(PLAN8_THREADS) void int8_plan_kernel(const int64_t*
             if (fault & 1) fault = 1;
             bad |= fault;
         }
-        pos_of[a] = fault ? -1 : atomicAdd(&count[e], 1);      // (the rank; its expert's start is added below)
+        return fault ? -1 : atomicAdd(&count[e], 1);
+    };
+#pragma unroll
+    for (int j = 0; j < NR; ++j) {
+        const int a = tid + j * PLAN8_THREADS;
+        mine[j] = 0;
+        rank[j] = -1;
+        if (j * PLAN8_THREADS < assignments) {
+            const int64_t e = ldg<int64_t>(ids + (a < assignments ? a : 0));
+            if (a < assignments) rank[j] = count_in(a, e);
+            mine[j] = rank[j] < 0 ? 0 : (int)e;
+        }
     }
+    for (int a = tid + NR * PLAN8_THREADS; a < assignments; a += PLAN8_THREADS) pos_of[a] = count_in(a, ldg<int64_t>(ids + a));
     if (bad && status_out) atomicOr(status_out, bad);
     __syncthreads();
     const int per = (n_experts + PLAN8_THREADS - 1) / PLAN8_THREADS, e0 = tid * per;
@@ -129,10 +158,18 @@ __global__ __launch_bounds__(PLAN8_THREADS) void int8_plan_kernel(const int64_t*
         upto += count[e];
     }
     __syncthreads();
-    for (int a = tid; a < assignments; a += PLAN8_THREADS) {
-        const int rank = pos_of[a];              // (written by this thread)
-        if (rank < 0) continue;
-        const int p = start[ldg<int64_t>(ids + a)] + rank;
+#pragma unroll
+    for (int j = 0; j < NR; ++j) {
+        const int a = tid + j * PLAN8_THREADS;
+        if (a >= assignments) break;
+        const int p = rank[j] < 0 ? -1 : start[mine[j]] + rank[j];
+        pos_of[a] = p;
+        if (p >= 0) row_of[p] = a / k;
+    }
+    for (int a = tid + NR * PLAN8_THREADS; a < assignments; a += PLAN8_THREADS) {
+        const int r = pos_of[a];                 // (written by this thread)
+        if (r < 0) continue;
+        const int p = start[ldg<int64_t>(ids + a)] + r;
         pos_of[a] = p;
         row_of[p] = a / k;
     }
@@ -293,7 +330,7 @@ static Int8MoeLayout int8_moe_layout(int tokens, int k, int n_experts, int d, in
 }
 
 static size_t int8_moe_bytes(int tokens, int k, int n_experts, int d, int f, int fs) {
-    return int8_step_covers(tokens, k, n_experts, d, f, fs) ? int8_step_bytes(tokens, k, f, fs)
+    return int8_step_covers(tokens, k, n_experts, d, f, fs) ? int8_step_bytes(tokens, k, d, f, fs)
                                                              : int8_moe_layout(tokens, k, n_experts, d, f, fs).total;
 }
 
@@ -304,16 +341,7 @@ static int int8_moe_impl(const qmoe_int8_moe_args& m, char* ws, const Int8MoeLay
     float* const weights = (float*)(ws + L.weights);
     int64_t* const ids = (int64_t*)(ws + L.ids);
     const int64_t dp = int8_cols256(d), fp = int8_cols256(f);
-    const int fast = (uintptr_t)m.hidden % 16 == 0 && d % 8 == 0;
-#define QMOE_INT8_ROUTE(DT)                                                                                                            \
-    hipLaunchKernelGGL((e <= 1024 ? int8_route_kernel<DT, 16> : int8_route_kernel<DT, 64>), dim3(t), dim3(320), 0, s, m.hidden, d, fast, \
-                       m.logits, e, k, m.floor_value, m.renormalize, m.in_weights, m.in_ids, weights, ids, m.out_weights, m.out_ids,     \
-                       (uint8_t*)(ws + L.q), dp, (float*)(ws + L.s))
-    if (m.hidden_dtype == QMOE_DT_F32) QMOE_INT8_ROUTE(QMOE_DT_F32);
-    else if (m.hidden_dtype == QMOE_DT_F16) QMOE_INT8_ROUTE(QMOE_DT_F16);
-    else QMOE_INT8_ROUTE(QMOE_DT_BF16);
-#undef QMOE_INT8_ROUTE
-    if ((rc = check_launch("int8 expert step (routing)"))) return rc;
+    if ((rc = int8_route_launch(m, weights, ids, (uint8_t*)(ws + L.q), dp, (float*)(ws + L.s), s))) return rc;
     const int rows = int8_plan_rows(a, e);
     hipLaunchKernelGGL(int8_plan_kernel, dim3(1), dim3(PLAN8_THREADS), (size_t)e * 8, s, ids, a, k, e, rows, m.logits ? 0 : 1, (int*)(ws + L.row_of),
                        (int*)(ws + L.pos_of), (int*)(ws + L.chunk_expert), (int*)(ws + L.chunk_start), (int*)(ws + L.chunk_count),

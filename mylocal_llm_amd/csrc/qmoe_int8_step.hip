@@ -14,6 +14,8 @@
 
 namespace qmoe {
 
+// Up to this many tokens every workgroup makes what it needs itself, beyond them launches of their own do it once.
+static constexpr int STEP8_FUSED = 4;
 static constexpr int STEP8_TOKENS = 16, STEP8_EXPERTS = 1024, STEP8_PAIRS = STEP8_TOKENS * 32;
 static constexpr int FRONT8_RING = 4;
 static constexpr int BACK8_WAVES = 16, BACK8_THREADS = 64 * BACK8_WAVES, BACK8_RING = 8;
@@ -37,6 +39,8 @@ struct Step8Between {
 
 struct Front8Args {
     const void* x;
+    const uint8_t* q;        // [tokens][kp] codes of x and their scales, where they are made beforehand
+    const float* q_scale;
     int tokens, k, n_experts, fast;
     const float* logits;
     float floor_value;
@@ -131,7 +135,8 @@ template <int NV> struct RowIds {
     }
 };
 
-template <int XDT, int WAVES>
+// CODED: routing and codes of the rows are there (int8_route_launch); in_ids and in_weights hold them.
+template <int XDT, int WAVES, bool CODED>
 __global__ __launch_bounds__(64 * WAVES) void int8_front_kernel(const Front8Args a) {
     extern __shared__ __align__(16) uint8_t dynamic[];      // [tokens][kp + 16] codes | [held][tokens][32] sums | [held][32] scales
     __shared__ uint32_t chosen[STEP8_EXPERTS];              // bit t: token t chose the expert
@@ -151,7 +156,7 @@ __global__ __launch_bounds__(64 * WAVES) void int8_front_kernel(const Front8Args
 
     // ---- requests: a wave's row of logits, eight values of x a thread and turn, up to NX turns in registers ----
     RowIds<8> narrow;
-    if (a.logits && wave < tokens) narrow.load(a.logits + (size_t)wave * a.n_experts, a.n_experts);
+    if (!CODED && a.logits && wave < tokens) narrow.load(a.logits + (size_t)wave * a.n_experts, a.n_experts);
     const int per = a.kp / 8, groups = tokens * per;
     constexpr int NX = 4;
     float v[NX][8];
@@ -159,9 +164,21 @@ __global__ __launch_bounds__(64 * WAVES) void int8_front_kernel(const Front8Args
         const int t = gi < groups ? over(gi, a.per_magic) : 0, i = (gi - t * per) * 8, left = gi < groups ? a.d - i : 0;
         int8_load8<XDT>(a.x, left > 0 ? (size_t)t * a.d + i : 0, left, a.fast, to);
     };
+    i32x4_t piece[NX];
+    const int pieces = tokens * per / 2;
+    auto fetch = [&](int p0) {
 #pragma unroll
-    for (int p = 0; p < NX; ++p)
-        if (p * THREADS < groups) load(p * THREADS + tid, v[p]);
+        for (int j = 0; j < NX; ++j) {
+            const int p = p0 + j * THREADS + tid;
+            piece[j] = ldg_i32x4(a.q + (int64_t)(p < pieces ? p : 0) * 16);
+        }
+    };
+    if (CODED) fetch(0);
+    else {
+#pragma unroll
+        for (int p = 0; p < NX; ++p)
+            if (p * THREADS < groups) load(p * THREADS + tid, v[p]);
+    }
     for (int i = tid; i < a.n_experts; i += THREADS) chosen[i] = 0u;
     if (tid < STEP8_TOKENS) tops[tid] = 0u;
     for (int i = tid; i < a.held * tokens * 32; i += THREADS) sums[i] = 0;
@@ -186,27 +203,40 @@ __global__ __launch_bounds__(64 * WAVES) void int8_front_kernel(const Front8Args
             f(g0 + tid, w);
         }
     };
-    turns(raise);
-    meet_lds();
+    if (!CODED) {
+        turns(raise);
+        meet_lds();
+    }
 
     // ---- codes ----
-    if (tid < tokens) srow[tid] = RowScale(tops[tid]).s;
-    turns([&](int gi, const float* w) {
-        const int t = gi < groups ? over(gi, a.per_magic) : 0, i = (gi - t * per) * 8;
-        const u32x2_t q = int8_code8(w, RowScale(tops[t]));
-        if (gi < groups) *(u32x2_t*)(codes + t * stride + i) = q;
-    });
+    if (tid < tokens) srow[tid] = CODED ? ldg<float>(a.q_scale + tid) : RowScale(tops[tid]).s;
+    if (CODED) {
+        for (int p0 = 0; p0 < pieces; p0 += NX * THREADS) {
+#pragma unroll
+            for (int j = 0; j < NX; ++j) {
+                const int p = p0 + j * THREADS + tid, t = over(2 * p, a.per_magic);
+                if (p < pieces) *(i32x4_t*)(codes + t * stride + (2 * p - t * per) * 8) = piece[j];
+            }
+            if (p0 + NX * THREADS < pieces) fetch(p0 + NX * THREADS);
+        }
+    } else {
+        turns([&](int gi, const float* w) {
+            const int t = gi < groups ? over(gi, a.per_magic) : 0, i = (gi - t * per) * 8;
+            const u32x2_t q = int8_code8(w, RowScale(tops[t]));
+            if (gi < groups) *(u32x2_t*)(codes + t * stride + i) = q;
+        });
+    }
     // ---- routing: a wave a token ----
     int bad = 0;
     for (int t = wave; t < tokens; t += WAVES) {
         const float* const z = a.logits + (size_t)t * a.n_experts;
         float weight = 0.0f;
         int64_t id = -1;
-        if (a.logits && publisher) router_row<16>(z, a.n_experts, k, a.floor_value, a.renorm, weight, id, [] {});
-        else if (a.logits && a.n_experts <= 512) {
+        if (!CODED && a.logits && publisher) router_row<16>(z, a.n_experts, k, a.floor_value, a.renorm, weight, id, [] {});
+        else if (!CODED && a.logits && a.n_experts <= 512) {
             if (t != wave) narrow.load(z, a.n_experts);
             id = narrow.select(a.n_experts, k, (uint2*)slot_of + wave * 64);
-        } else if (a.logits) {
+        } else if (!CODED && a.logits) {
             RowIds<16> wide;
             wide.load(z, a.n_experts);
             id = wide.select(a.n_experts, k, (uint2*)slot_of + wave * 64);
@@ -426,7 +456,6 @@ struct Back8Args {
 
 // The hidden activations' codes for more than STEP8_FUSED tokens, a workgroup a row: a workgroup of the back kernel that makes
 // them itself needs 15 us for 16 tokens (every one makes all of them), this launch and reading its codes 4 us.
-static constexpr int STEP8_FUSED = 4;
 __global__ __launch_bounds__(256) void int8_hidden_codes_kernel(const Back8Args a) {
     __shared__ uint32_t tops[4];
     const int pairs = a.tokens * a.k, r = blockIdx.x, tid = threadIdx.x;
@@ -665,8 +694,8 @@ template <bool CODES> __global__ __launch_bounds__(BACK8_THREADS) void int8_back
 }
 
 // ---- host --------------------------------------------------------------------------------------------------
-struct Step8Layout { size_t h, h_top, sh, sh_top, admit, weight, kept, n_active, active, slot, row_codes, row_scale, total; };
-static Step8Layout step8_layout(int tokens, int k, int f, int fs) {
+struct Step8Layout { size_t h, h_top, sh, sh_top, admit, weight, kept, n_active, active, slot, row_codes, row_scale, q, q_scale, ids, total; };
+static Step8Layout step8_layout(int tokens, int k, int d, int f, int fs) {
     Step8Layout w;
     size_t at = 0;
     const size_t pairs = (size_t)tokens * k;
@@ -683,6 +712,9 @@ static Step8Layout step8_layout(int tokens, int k, int f, int fs) {
     w.slot = take(pairs * STEP8_TOKENS);
     w.row_codes = take(pairs * int8_cols64(f) + (size_t)tokens * (fs ? int8_cols64(fs) : 0));
     w.row_scale = take((pairs + tokens) * 4);
+    w.q = take(tokens * int8_cols64(d));
+    w.q_scale = take(tokens * 4);
+    w.ids = take(pairs * 8);
     w.total = at;
     return w;
 }
@@ -703,7 +735,7 @@ bool int8_step_covers(int tokens, int k, int n_experts, int d, int f, int fs) {
     return tokens <= STEP8_TOKENS && k <= 32 && n_experts <= STEP8_EXPERTS && back8_lds(tokens, k, f, fs) <= STEP8_LDS &&
            front8_codes(tokens, d) + 4 * front8_item(tokens) <= STEP8_LDS;
 }
-size_t int8_step_bytes(int tokens, int k, int f, int fs) { return step8_layout(tokens, k, f, fs).total; }
+size_t int8_step_bytes(int tokens, int k, int d, int f, int fs) { return step8_layout(tokens, k, d, f, fs).total; }
 
 static int raise_lds(const void* fn, bool (&raised)[64]) {
     int dev = 0;
@@ -715,14 +747,14 @@ static int raise_lds(const void* fn, bool (&raised)[64]) {
     return QMOE_OK;
 }
 
-template <int XDT, int WAVES> static int front8_as(const Front8Args& a, int grid, size_t lds, hipStream_t s) {
+template <int XDT, int WAVES, bool CODED> static int front8_as(const Front8Args& a, int grid, size_t lds, hipStream_t s) {
     static bool raised[64];
-    if (const int rc = raise_lds((const void*)&int8_front_kernel<XDT, WAVES>, raised)) return rc;
-    hipLaunchKernelGGL((int8_front_kernel<XDT, WAVES>), dim3(grid), dim3(64 * WAVES), lds, s, a);
+    if (const int rc = raise_lds((const void*)&int8_front_kernel<XDT, WAVES, CODED>, raised)) return rc;
+    hipLaunchKernelGGL((int8_front_kernel<XDT, WAVES, CODED>), dim3(grid), dim3(64 * WAVES), lds, s, a);
     return check_launch("int8 expert step (front)");
 }
 template <int XDT> static int front8_waves(const Front8Args& a, int grid, size_t lds, hipStream_t s) {
-    return a.tokens <= 4 ? front8_as<XDT, 8>(a, grid, lds, s) : front8_as<XDT, 16>(a, grid, lds, s);
+    return a.tokens <= STEP8_FUSED ? front8_as<XDT, 8, false>(a, grid, lds, s) : front8_as<XDT, 16, true>(a, grid, lds, s);
 }
 static uint32_t magic_of(int d) { return d <= 1 ? 0u : (uint32_t)(0x100000000ull / (uint32_t)d) + 1u; }
 
@@ -734,10 +766,11 @@ template <bool CODES> static int back8_as(const Back8Args& a, hipStream_t s) {
 }
 
 int stream_grid();
+int int8_route_launch(const qmoe_int8_moe_args& m, float* weights, int64_t* ids, uint8_t* codes, int64_t ld, float* scales, hipStream_t s);
 
 int int8_step_launch(const qmoe_int8_moe_args& m, char* ws, hipStream_t s) {
     const int t = m.tokens, k = m.top_k, d = m.d_model, f = m.d_ff, fs = m.d_ff_shared;
-    const Step8Layout L = step8_layout(t, k, f, fs);
+    const Step8Layout L = step8_layout(t, k, d, f, fs);
     Step8Between b{(float*)(ws + L.h), (uint32_t*)(ws + L.h_top), (float*)(ws + L.sh), (uint32_t*)(ws + L.sh_top), (float*)(ws + L.admit),
                    (float*)(ws + L.weight), (int*)(ws + L.kept), (int*)(ws + L.n_active), (int*)(ws + L.active), (uint8_t*)(ws + L.slot),
                    (uint8_t*)(ws + L.row_codes), (float*)(ws + L.row_scale)};
@@ -762,6 +795,16 @@ int int8_step_launch(const qmoe_int8_moe_args& m, char* ws, hipStream_t s) {
     a.held = (int)(need < fits ? need : fits);
     const size_t lds = codes + a.held * front8_item(t);
     int rc;
+    if (t > STEP8_FUSED) {
+        a.q = (const uint8_t*)(ws + L.q);
+        a.q_scale = (const float*)(ws + L.q_scale);
+        a.in_ids = (const int64_t*)(ws + L.ids);
+        a.in_weights = b.weight;
+        if ((rc = int8_route_launch(m, b.weight, (int64_t*)(ws + L.ids), (uint8_t*)(ws + L.q), a.kp, (float*)(ws + L.q_scale), s))) return rc;
+        a.logits = nullptr;
+        a.out_weights = nullptr;
+        a.out_ids = nullptr;
+    }
     if (m.hidden_dtype == QMOE_DT_F32) rc = front8_waves<QMOE_DT_F32>(a, grid, lds, s);
     else if (m.hidden_dtype == QMOE_DT_F16) rc = front8_waves<QMOE_DT_F16>(a, grid, lds, s);
     else rc = front8_waves<QMOE_DT_BF16>(a, grid, lds, s);
