@@ -5,7 +5,7 @@
 //   (q, s) = codes of the hidden rows;  h = fl32(silu(g) u) per assignment;  (hq, hs) = codes of h;
 //   term = down;  out[t] = residual + (((0 + w_1 term_1) + w_2 term_2) + ... + sigmoid(x . gate) shared), experts
 //   in ascending id, each product rounded before it is added.
-#include "qmoe_int8.hpp"
+#include "qmoe_int8_route.hpp"
 
 namespace qmoe {
 
@@ -32,7 +32,13 @@ __global__ __launch_bounds__(320) void int8_route_kernel(const void* __restrict_
     if (tid < 0) {
         float w = 0.0f;
         int64_t id = 0;
-        if (logits) router_row<NV>(logits + t * n_experts, n_experts, k, floor_value, renorm, w, id, [] {});
+        const float* const z = logits + t * n_experts;
+        if (logits && NV <= 16) {
+            __shared__ uint2 scratch[64];
+            RowIds<NV <= 16 ? NV : 16> row;
+            row.load(z, n_experts);
+            row.route(z, n_experts, k, floor_value, renorm, scratch, w, id);
+        } else if (logits) router_row<NV>(z, n_experts, k, floor_value, renorm, w, id, [] {});
         else if (lane < k) {
             w = ldg<float>(in_weights + t * k + lane);
             id = ldg<int64_t>(in_ids + t * k + lane);
@@ -79,7 +85,7 @@ int int8_route_launch(const qmoe_int8_moe_args& m, float* weights, int64_t* ids,
     const int t = m.tokens, k = m.top_k, e = m.n_experts, d = m.d_model;
     const int fast = (uintptr_t)m.hidden % 16 == 0 && d % 8 == 0;
 #define QMOE_INT8_ROUTE(DT)                                                                                                              \
-    hipLaunchKernelGGL((e <= 1024 ? int8_route_kernel<DT, 16> : int8_route_kernel<DT, 64>), dim3(t), dim3(320), 0, s, m.hidden, d, fast, \
+    hipLaunchKernelGGL((e <= 512 ? int8_route_kernel<DT, 8> : e <= 1024 ? int8_route_kernel<DT, 16> : int8_route_kernel<DT, 64>), dim3(t), dim3(320), 0, s, m.hidden, d, fast, \
                        m.logits, e, k, m.floor_value, m.renormalize, m.in_weights, m.in_ids, weights, ids, m.out_weights, m.out_ids,     \
                        codes, ld, scales)
     if (m.hidden_dtype == QMOE_DT_F32) QMOE_INT8_ROUTE(QMOE_DT_F32);

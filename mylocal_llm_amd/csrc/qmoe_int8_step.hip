@@ -10,7 +10,7 @@
 // 64 columns are one list, cut evenly over its waves whatever expert they belong to; where a wave leaves an expert it adds
 // its partial sums to LDS as integers, so neither the cut nor the order of the waves changes a bit, and no wave waits for
 // another inside the stream.  Requests run R steps ahead through a ring of registers.
-#include "qmoe_int8.hpp"
+#include "qmoe_int8_route.hpp"
 
 namespace qmoe {
 
@@ -61,79 +61,6 @@ struct Front8Args {
 
 // x / d for x * d < 2^32; magic = floor(2^32 / d) + 1 (d > 1), 0 for d = 1
 __host__ __device__ __forceinline__ int over(int x, uint32_t magic) { return magic ? (int)(((uint64_t)(uint32_t)x * magic) >> 32) : x; }
-
-// The k largest of a row held NV values a lane, as RouterRow::select picks them (descending, NaN last, lower id on ties):
-// lane s gets selection s.  The weights are made by one workgroup alone: nothing but the ids is needed to stream.
-template <int NV> struct RowIds {
-    float v[NV];
-    __device__ __forceinline__ void load(const float* z, int n) {
-        const int lane = threadIdx.x & 63;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) v[j] = ldg<float>(z + (lane + 64 * j < n ? lane + 64 * j : 0));
-    }
-    // The k-th largest of the lanes' largest keys is a bound that at least k keys reach, and hardly more: those are gathered,
-    // one a lane, and ranked.  (k rounds of "largest of the wave, take it out" cost 4.5 us for ten of 512, this one fifth.)
-    // More than 64 keys reach the bound only where many are equal: then the rounds.  `scratch`: 64 entries of this wave.
-    __device__ __forceinline__ int select(int n, int k, uint2* scratch) {
-        const int lane = threadIdx.x & 63;
-        uint32_t key[NV], top = 0u;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const uint32_t o = order_key(v[j]);
-            key[j] = lane + 64 * j < n ? (o ? o : 1u) : 0u;
-            top = key[j] > top ? key[j] : top;
-        }
-        int ahead = 0;
-#pragma unroll
-        for (int i = 0; i < 64; ++i) ahead += (uint32_t)__builtin_amdgcn_readlane((int)top, i) > top;
-        uint32_t bound = ~wave_max_u32(ahead < k ? ~top : 0u);
-        bound = bound ? bound : 1u;
-        int count = 0;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const bool in = key[j] >= bound;
-            const unsigned long long m = __ballot(in);
-            const int at = count + __popcll(m & ((1ull << lane) - 1));
-            if (in && at < 64) scratch[at] = make_uint2(key[j], (uint32_t)(lane + 64 * j));
-            count += __popcll(m);
-        }
-        if (__builtin_expect(count > 64, 0)) return rounds(key, k);
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
-        // (gathered in ascending id: among equal keys the lower lane comes first)
-        const uint2 mine = lane < count ? scratch[lane] : make_uint2(0u, 0u);
-        int rank = 0;
-        for (int i = 0; i < count; ++i) {
-            const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)mine.x, i);
-            rank += other > mine.x || (other == mine.x && i < lane);
-        }
-        return __builtin_amdgcn_ds_permute((lane < count ? rank : lane) * 4, (int)mine.y);
-    }
-    __device__ __forceinline__ static int rounds(uint32_t (&key)[NV], int k) {
-        const int lane = threadIdx.x & 63;
-        int mine = 0;
-        for (int slot = 0; slot < k; ++slot) {
-            uint32_t c = 0u;
-#pragma unroll
-            for (int j = 0; j < NV; ++j) c = key[j] > c ? key[j] : c;
-            const uint32_t win = wave_max_u32(c);
-            int wj = 0;
-            unsigned long long holders = 0ull;
-#pragma unroll
-            for (int j = NV - 1; j >= 0; --j) {
-                const unsigned long long b = __ballot(key[j] == win);
-                if (b) { wj = j; holders = b; }
-            }
-            const int wl = __builtin_ctzll(holders);
-#pragma unroll
-            for (int j = 0; j < NV; ++j)
-                if (j == wj) key[j] = lane == wl ? 0u : key[j];
-            if (lane == slot) mine = wl + 64 * wj;
-        }
-        return mine;
-    }
-};
 
 // CODED: routing and codes of the rows are there (int8_route_launch); in_ids and in_weights hold them.
 template <int XDT, int WAVES, bool CODED>
@@ -232,14 +159,17 @@ __global__ __launch_bounds__(64 * WAVES) void int8_front_kernel(const Front8Args
         const float* const z = a.logits + (size_t)t * a.n_experts;
         float weight = 0.0f;
         int64_t id = -1;
-        if (!CODED && a.logits && publisher) router_row<16>(z, a.n_experts, k, a.floor_value, a.renorm, weight, id, [] {});
-        else if (!CODED && a.logits && a.n_experts <= 512) {
+        uint2* const scratch = (uint2*)slot_of + wave * 64;
+        // (nothing but the ids is needed to stream: one workgroup makes the weights)
+        if (!CODED && a.logits && a.n_experts <= 512) {
             if (t != wave) narrow.load(z, a.n_experts);
-            id = narrow.select(a.n_experts, k, (uint2*)slot_of + wave * 64);
+            if (publisher) narrow.route(z, a.n_experts, k, a.floor_value, a.renorm, scratch, weight, id);
+            else id = narrow.select(a.n_experts, k, scratch);
         } else if (!CODED && a.logits) {
             RowIds<16> wide;
             wide.load(z, a.n_experts);
-            id = wide.select(a.n_experts, k, (uint2*)slot_of + wave * 64);
+            if (publisher) wide.route(z, a.n_experts, k, a.floor_value, a.renorm, scratch, weight, id);
+            else id = wide.select(a.n_experts, k, scratch);
         } else if (lane < k) {
             weight = ldg<float>(a.in_weights + (size_t)t * k + lane);
             id = ldg<int64_t>(a.in_ids + (size_t)t * k + lane);

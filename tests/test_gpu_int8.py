@@ -305,6 +305,28 @@ def test_step_from_logits(cuda, t, e, k, d, f, fs, dtype):
     assert torch.equal(again, got) and torch.equal(w2, w) and torch.equal(ids2, ids)
 
 
+@pytest.mark.parametrize("t", [1, 3, 12, 40])
+@pytest.mark.parametrize("e,k", [(3, 3), (64, 8), (512, 10), (700, 32), (1024, 1), (1500, 7), (4096, 4)])
+def test_routing_order_ties_infinities_and_nan(cuda, t, e, k):
+    """Rows of equal logits, of few distinct values, with infinities and NaN: ids equal the router's everywhere."""
+    announce("int8 routing", t, e, k)
+    d, f = 64, 16
+    bank, _, _ = layer(e, d, f, 0, 1) if e <= 700 else (tuple((torch.ones((e, *s), dtype=torch.int8, device=cuda), torch.full((e, s[0]), 1e-3, device=cuda))
+                                                              for s in ((f, d), (f, d), (d, f))), None, None)
+    dev = Int8ExpertBank(*bank)
+    rng = np.random.default_rng(e + t)
+    kinds = [np.zeros((t, e)), rng.integers(0, 3, (t, e)), rng.standard_normal((t, e)), np.where(rng.random((t, e)) < 0.3, -np.inf, rng.standard_normal((t, e))),
+             np.where(rng.random((t, e)) < 0.2, np.nan, rng.standard_normal((t, e))), np.full((t, e), -np.inf), -np.abs(rng.standard_normal((t, e))) * 1e-30]
+    x = rows(t, d, 1)
+    for z in kinds:
+        z = z.astype(np.float32)
+        _, w, ids = int8_moe_step(x, dev, k, logits=torch.from_numpy(z).cuda(), return_routing=True)
+        with np.errstate(all="ignore"):
+            want_w, want_ids = R.router_topk(z, k)
+        np.testing.assert_array_equal(ids.cpu().numpy(), want_ids)
+        np.testing.assert_allclose(w.cpu().numpy(), want_w, rtol=2e-6, atol=2e-7, equal_nan=True)
+
+
 @pytest.mark.parametrize("t", [1, 6, 16, 50])
 def test_step_with_bad_ids_repeats_and_rows(cuda, t):
     e, k, d, f = 12, 4, 160, 96
