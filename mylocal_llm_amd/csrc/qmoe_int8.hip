@@ -83,6 +83,11 @@ __global__ __launch_bounds__(1024) void int8_quantize_long_kernel(const void* __
 }
 
 template <int DT> static int quantize_as(const void* x, int64_t rows, int k, uint8_t* codes, int64_t ld, int width, float* scales, hipStream_t s) {
+    constexpr int64_t MOST = 4000000;      // rows of a launch: its threads are counted in 32 bits
+    if (rows > MOST) {
+        if (const int rc = quantize_as<DT>(x, MOST, k, codes, ld, width, scales, s)) return rc;
+        return quantize_as<DT>((const char*)x + MOST * k * (int64_t)sizeof(typename Elem<DT>::T), rows - MOST, k, codes + MOST * ld, ld, width, scales + MOST, s);
+    }
     const dim3 grid((unsigned)rows);
     const int eights = (width + 7) / 8;
     if (eights > 2048) {
@@ -151,6 +156,7 @@ static int dense(const char* who, bool pair, const void* w, const float* c, cons
     if ((uintptr_t)w % 16 || (pair && (uintptr_t)w2 % 16) || (uintptr_t)c % 4 || (pair && (uintptr_t)c2 % 4) || (uintptr_t)xs % 4 ||
         (xdt != QMOE_DT_I8 && (uintptr_t)x % dtype_size(xdt)) || (uintptr_t)y % dtype_size(ydt))
         return fail(QMOE_EINVAL, "%s: misaligned pointer", who);
+    if (n > (1 << 26) || tokens > (1 << 22)) return fail(QMOE_EUNSUPPORTED, "%s: more than 2^26 channels or 2^22 tokens; split the call", who);
     if (tokens == 0) return QMOE_OK;
     const size_t need = qmoe_int8_workspace_bytes(n, k, tokens, xdt);
     const bool direct = xdt == QMOE_DT_I8 && codes_as_they_are(x, k);
@@ -203,7 +209,7 @@ int qmoe_int8_tiles(const void* codes, int64_t matrices, int n, int k, void* til
     if (k > INT8_MAX_K) return fail(QMOE_EUNSUPPORTED, "%s: K=%d beyond %d, where an int32 sum could overflow", who, k, INT8_MAX_K);
     if ((uintptr_t)tiles % 16) return fail(QMOE_EINVAL, "%s: tiles must be 16-byte aligned", who);
     const int row_tiles = (int)(int8_rows16(n) / 16);
-    if (matrices * row_tiles > INT32_MAX) return fail(QMOE_EUNSUPPORTED, "%s: more than 2^31 - 1 rows of tiles; lay the matrices out in parts", who);
+    if (matrices > ((1 << 24) - 1) / row_tiles) return fail(QMOE_EUNSUPPORTED, "%s: 2^24 or more rows of tiles; lay the matrices out in parts", who);
     hipLaunchKernelGGL(int8_tiles_kernel, dim3((unsigned)(matrices * row_tiles)), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)codes, n, k,
                        row_tiles, (uint8_t*)tiles);
     return check_launch(who);

@@ -233,7 +233,7 @@ template <bool PAIR, bool HIDDEN, bool PLAN, int WN, int WT, int RT, int TT, int
 static int gemm8_as(const Int8Product& a, int chunks, hipStream_t s, const Int8Product* side = nullptr) {
     const int nb = (a.n + 16 * WN * RT - 1) / (16 * WN * RT), tb = PLAN ? (chunks + 31) / 32 * 32 : (a.tokens + 16 * WT * TT - 1) / (16 * WT * TT);
     const int sn = side ? (side->n + 16 * WN * RT - 1) / (16 * WN * RT) : 0, st = side ? (side->tokens + 16 * WT * TT - 1) / (16 * WT * TT) : 0;
-    if ((int64_t)nb * tb + (int64_t)sn * st > INT32_MAX)
+    if (((int64_t)nb * tb + (int64_t)sn * st) * (64 * WN * WT) > 0xFFFFFFFFll)      // (a launch's threads are counted in 32 bits)
         return fail(QMOE_EUNSUPPORTED, "int8 product: %d x %d blocks exceed a launch; split the tokens", nb, tb);
     hipLaunchKernelGGL((int8_gemm_kernel<PAIR, HIDDEN, PLAN, WN, WT, RT, TT, KC, R>), dim3(nb * tb + sn * st), dim3(64 * WN * WT), 0, s, a, nb, PLAN ? chunks : tb,
                        side ? *side : a, sn, st);

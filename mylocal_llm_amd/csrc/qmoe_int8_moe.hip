@@ -406,7 +406,7 @@ static int int8_moe_check(const qmoe_int8_moe_args& m) {
     if (m.d_model < 1 || m.d_ff < 1 || m.d_ff_shared < 0) return fail(QMOE_EINVAL, "%s: bank dimensions must be positive", who);
     if (m.d_model > INT8_MAX_K || m.d_ff > INT8_MAX_K || m.d_ff_shared > INT8_MAX_K)
         return fail(QMOE_EUNSUPPORTED, "%s: a width beyond %d, where an int32 sum could overflow", who, INT8_MAX_K);
-    if ((int64_t)m.tokens * m.top_k > INT32_MAX / 2) return fail(QMOE_EUNSUPPORTED, "%s: too many assignments; split the tokens", who);
+    if ((int64_t)m.tokens * m.top_k > (1 << 22)) return fail(QMOE_EUNSUPPORTED, "%s: more than 2^22 assignments; split the tokens", who);
     const void* tiles[6] = {m.gate, m.up, m.down, m.shared_gate_w, m.shared_up_w, m.shared_down_w};
     const float* scales[6] = {m.gate_scales, m.up_scales, m.down_scales, m.shared_gate_scales, m.shared_up_scales, m.shared_down_scales};
     bool any = false;

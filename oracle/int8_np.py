@@ -16,8 +16,8 @@ def quantize(x):
 
 def product(q, s, w, c):
     """sum_k q w (exact) * s * c in 64 bits; q [T, K], w [N, K] whole numbers."""
-    acc = q.astype(np.int64) @ np.asarray(w).astype(np.int64).T
-    return acc.astype(np.float64) * (np.asarray(s, np.float64)[:, None] * np.asarray(c, np.float64)[None, :])
+    acc = np.asarray(q, np.float64) @ np.asarray(w, np.float64).T        # (whole numbers below 2^53: exact in any order)
+    return acc * (np.asarray(s, np.float64)[:, None] * np.asarray(c, np.float64)[None, :])
 
 
 def swish(g, u):

@@ -46,7 +46,7 @@ def rows(t, k, seed, dtype=torch.float32, device="cuda"):
 
 def matrix(n, k, seed, lead=(), device="cuda"):
     rng = np.random.default_rng(seed)
-    codes = rng.integers(-127, 128, (*lead, n, k)).astype(np.int8)
+    codes = rng.integers(-127, 128, (*lead, n, k), dtype=np.int8)
     scales = (rng.random((*lead, n)) * 1e-3 + 1e-4).astype(np.float32)
     return torch.from_numpy(codes).to(device), torch.from_numpy(scales).to(device)
 
@@ -125,7 +125,7 @@ def test_views_at_odd_addresses_and_higher_ranks(cuda):
 
 SHAPES = [(1, 1, 1), (1, 16, 64), (1, 17, 65), (1, 4096, 512), (2, 15, 63), (3, 100, 129), (5, 33, 1000), (15, 48, 4096), (16, 64, 192), (17, 250, 128),
           (31, 1, 257), (33, 129, 320), (48, 272, 511), (64, 144, 640), (65, 16, 64), (77, 1001, 1234), (100, 300, 96), (128, 256, 256),
-          (129, 257, 257), (200, 64, 2048), (256, 512, 128), (300, 520, 448), (513, 130, 200), (1, 32, 14336), (4, 32, 20000), (40, 32, 14336)]
+          (129, 257, 257), (200, 64, 2048), (256, 512, 128), (300, 520, 448), (513, 130, 200), (1, 32, 14336), (1, 33, 16385), (4, 32, 20000), (40, 32, 14336), (700, 700, 320), (300, 16 * 300, 64)]
 
 
 @pytest.mark.parametrize("t,n,k", SHAPES)
@@ -282,7 +282,8 @@ CASES = [  # tokens, experts, top_k, d_model, d_ff, d_shared
     (1, 4, 1, 64, 64, 0), (1, 16, 4, 256, 128, 256), (1, 512, 10, 2048, 512, 2048), (2, 8, 8, 100, 50, 30), (3, 7, 3, 65, 33, 0),
     (4, 32, 2, 192, 1536, 64), (5, 60, 4, 128, 704, 100), (9, 512, 10, 256, 64, 0), (15, 5, 5, 330, 130, 17), (16, 64, 6, 512, 256, 512),
     (16, 2, 1, 64, 2048, 0), (17, 16, 4, 256, 256, 256), (33, 9, 2, 130, 70, 0), (64, 40, 8, 256, 100, 128), (100, 3, 3, 77, 91, 13), (200, 64, 2, 320, 192, 0),
-    (1, 8, 2, 4096, 300, 0), (7, 8, 2, 300, 4096, 0), (2, 4, 2, 8200, 80, 16)]
+    (1, 8, 2, 4096, 300, 0), (7, 8, 2, 300, 4096, 0), (2, 4, 2, 8200, 80, 16),
+    (16, 12, 2, 8128, 1500, 0), (17, 6, 2, 8128, 100, 40), (64, 8, 4, 192, 160, 96), (40, 2, 1, 64, 300, 0), (300, 3, 2, 128, 130, 50)]
 
 
 @pytest.mark.parametrize("t,e,k,d,f,fs", CASES)
@@ -450,6 +451,20 @@ def test_a_run_of_the_operators_replays_from_a_graph(cuda, t):
             assert torch.equal(out, eager)
 
 
+@pytest.mark.parametrize("t", [1, 4, 9, 16, 60])
+def test_the_same_call_gives_the_same_bits(cuda, t):
+    e, k, d, f, fs = 24, 4, 320, 192, 128
+    bank, shared, vec = layer(e, d, f, fs, 4)
+    dev, dshared = Int8ExpertBank(*bank), tuple(Int8Weight(*m) for m in shared)
+    x, logits = rows(t, d, 2), torch.from_numpy(synthetic.router_logits(t, e, 3)).cuda()
+    first = int8_moe_step(x, dev, k, logits=logits, shared=dshared, shared_gate=vec)
+    for _ in range(6):
+        assert torch.equal(int8_moe_step(x, dev, k, logits=logits, shared=dshared, shared_gate=vec), first)
+    order = torch.randperm(t)
+    moved = int8_moe_step(x[order].contiguous(), dev, k, logits=logits[order].contiguous(), shared=dshared, shared_gate=vec)
+    assert torch.equal(moved, first[order])          # a token's result does not depend on its place
+
+
 def test_calls_on_two_streams_do_not_meet(cuda):
     e, k, d, f = 32, 4, 256, 128
     bank, _, _ = layer(e, d, f, 0, 12)
@@ -467,6 +482,46 @@ def test_calls_on_two_streams_do_not_meet(cuda):
     torch.cuda.synchronize()
     for i, (a, b) in enumerate(got):
         assert torch.equal(a, want[i % 4][0]) and torch.equal(b, want[i % 4][1])
+
+
+@pytest.mark.parametrize("t,n,k", [(1, 64, 128), (20, 64, 128), (150, 256, 128), (130, 128, 256)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_outputs_at_odd_addresses(cuda, t, n, k, dtype):
+    """The C entry writes to any address that its element type allows; results equal the aligned ones."""
+    from mylocal_llm_amd import _lib
+    from mylocal_llm_amd.quantized_linear import _TORCH_DTYPE_ID
+    lib = _lib.load()
+    x, weight = rows(t, k, 3, dtype), Int8Weight(*matrix(n, k, 4))
+    want = int8_linear(x, weight)
+    base = torch.full((t * n + 2,), 3.0, dtype=dtype, device=cuda)
+    work = torch.empty(lib.qmoe_int8_workspace_bytes(n, k, t, 0) + 256, dtype=torch.uint8, device=cuda)
+    rc = lib.qmoe_int8_linear(weight.tiles.data_ptr(), weight.scales.data_ptr(), n, k, x.data_ptr(), _TORCH_DTYPE_ID[dtype], None, t,
+                              base[1:].data_ptr(), _TORCH_DTYPE_ID[dtype], work.data_ptr(), work.numel(), torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    torch.cuda.synchronize()
+    got = base[1:-1].reshape(t, n)
+    if dtype == torch.float32:
+        assert torch.equal(got, want)
+    else:                     # (fp32 or 64-bit scaling in front of the one rounding: a neighbour at most)
+        close(got, as_np(want), 4 * U)
+    assert base[0] == 3 and base[-1] == 3
+
+
+def test_many_short_rows_and_long_prompts_are_cut_into_launches(cuda):
+    x = torch.ones((4_000_003, 1), dtype=torch.float16, device=cuda)
+    x[-1] = -5.0
+    codes, scales = int8_quantize(x)
+    assert codes[:-1].eq(127).all() and codes[-1] == -127 and scales[-1].item() == np.float32(np.float64(5.0) / 127)
+    e, k, d, f = 6, 2, 64, 32
+    bank, _, _ = layer(e, d, f, 0, 2)
+    dev = Int8ExpertBank(*bank)
+    t = 9000                  # more than one call's worth of tokens
+    x, logits = rows(t, d, 1), torch.from_numpy(synthetic.router_logits(t, e, 3)).cuda()
+    got, w, ids = int8_moe_step(x, dev, k, logits=logits, return_routing=True)
+    at = torch.tensor([0, 1, 4095, 4096, 8191, 8192, 8999], device=cuda)
+    check_step(x[at], bank, None, None, w[at], ids[at], None, got[at])
+    part = int8_moe_step(x[4096:8192].contiguous(), dev, k, logits=logits[4096:8192].contiguous())
+    assert torch.equal(part, got[4096:8192])
 
 
 def test_rows_behind_the_output_are_left_alone(cuda):

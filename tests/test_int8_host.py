@@ -30,6 +30,7 @@ def test_linear_refuses_before_any_launch():
     assert linear(lib, xdt=3) == 1 and b"scales" in lib.qmoe_last_error()
     assert linear(lib, tiles=FAKE + 8) == 1 and linear(lib, x=FAKE + 2) == 1 and linear(lib, y=FAKE + 1) == 1
     assert linear(lib, t=2, ws=None) == 4 and linear(lib, t=2, ws=FAKE + 16) == 4 and linear(lib, t=2, bytes=64) == 4
+    assert linear(lib, n=1 << 27) == 2 and linear(lib, t=1 << 23) == 2
     assert linear(lib, t=0) == 0
 
 
@@ -41,7 +42,7 @@ def test_swiglu_quantise_and_tiles_refuse_before_any_launch():
     assert qz(x=None) == 1 and qz(c=None) == 1 and qz(s=None) == 1 and qz(dt=3) == 1 and qz(rows=-1) == 1 and qz(k=0) == 1
     assert qz(x=FAKE + 1) == 1 and qz(s=FAKE + 2) == 1 and qz(rows=1 << 33) == 2 and qz(rows=0) == 0
     tl = lambda c=FAKE, m=1, n=4, k=4, t=FAKE: lib.qmoe_int8_tiles(c, m, n, k, t, None)
-    assert tl(c=None) == 1 and tl(t=None) == 1 and tl(m=0) == 1 and tl(n=0) == 1 and tl(k=131072) == 2 and tl(t=FAKE + 4) == 1
+    assert tl(c=None) == 1 and tl(t=None) == 1 and tl(m=0) == 1 and tl(n=0) == 1 and tl(k=131072) == 2 and tl(t=FAKE + 4) == 1 and tl(m=1 << 30) == 2
 
 
 def test_sizes():
@@ -74,7 +75,7 @@ def test_step_refuses_before_any_launch():
     assert call(logits=None) == 1 and call(logits=None, in_weights=FAKE) == 1
     assert call(tokens=-1) == 1 and call(hidden_dtype=3) == 1 and call(out_dtype=9) == 1 and call(d_model=0) == 1 and call(d_ff=-4) == 1
     assert call(n_experts=4097) == 2 and call(top_k=0) == 2 and call(top_k=9) == 2 and call(top_k=33, n_experts=64) == 2
-    assert call(d_ff=131072) == 2 and call(tokens=1 << 30, top_k=2) == 2
+    assert call(d_ff=131072) == 2 and call(tokens=1 << 30, top_k=2) == 2 and call(tokens=(1 << 21) + 1, top_k=2) == 2
     assert call(d_ff_shared=16) == 1 and call(shared_gate_w=FAKE) == 1
     assert call(d_ff_shared=16, shared_gate_w=FAKE, shared_up_w=FAKE, shared_down_w=FAKE, shared_gate_scales=FAKE, shared_up_scales=FAKE) == 1
     assert call(floor_value=0.0) == 1 and call(floor_value=float("nan")) == 1
