@@ -295,6 +295,7 @@ int qmoe_read_probe(const void* buffer, size_t bytes, uint32_t match, uint32_t* 
  * counterpart in the reference, whose packed products keep activations in floating point.
  *     q[t, k] = rint(x[t, k] / s[t]),  s[t] = fl32(max_k |x[t, k]| / 127)   halves to even, |q| <= 127
  *     y[t, n] = (sum_k q[t, k] w[n, k]) * s[t] * c[n]                       int32 sum, exact
+ * in 64 bits and rounded to fp32, then to y's type (16-bit results of many tokens: scaled in fp32).
  * s[t] == 0 makes all codes 0; a row with a NaN or an infinity gets s[t] = NaN and codes of 0, so its
  * products are NaN.  Weights are any int8 codes with fp32 scales, laid out once as tiles of 16
  * channels x 64 columns (qmoe_int8_tiles), zero-padded.  K <= 131071, where the int32 sum cannot
@@ -316,7 +317,7 @@ int qmoe_int8_tiles(const void* codes, int64_t matrices, int n, int k, void* til
  * k % 256 == 0 at a 16-byte aligned address). */
 size_t qmoe_int8_workspace_bytes(int n, int k, int tokens, int x_dtype);
 
-/* y[tokens, n] as above, rounded once to y_dtype.  x: contiguous [tokens, k] in fp32 / fp16 / bf16,
+/* y[tokens, n] as above; at most 2^26 channels and 2^22 tokens a call.  x: contiguous [tokens, k] in fp32 / fp16 / bf16,
  * quantised on the way (x_scales ignored), or QMOE_DT_INT8 with x_scales[tokens]. */
 int qmoe_int8_linear(const void* tiles, const float* channel_scales, int n, int k, const void* x, int x_dtype,
                      const float* x_scales, int tokens, void* y, int y_dtype, void* workspace,

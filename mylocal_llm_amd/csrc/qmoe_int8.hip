@@ -35,7 +35,7 @@ __global__ __launch_bounds__(1024) void int8_quantize_kernel(const void* __restr
     for (int p = 0; p < NX; ++p)
 #pragma unroll
         for (int j = 0; j < 8; ++j) { const uint32_t b = abs_bits(v[p][j]); top = b > top ? b : top; }
-    top = wave_top(top);
+    top = wave_max_u32(top);
     if (threads > 64) {
         if ((tid & 63) == 0) tops[tid >> 6] = top;
         __syncthreads();
@@ -72,7 +72,7 @@ __global__ __launch_bounds__(1024) void int8_quantize_long_kernel(const void* __
         const uint32_t b = abs_bits(Elem<DT>::load(x, base + i));
         top = b > top ? b : top;
     }
-    top = wave_top(top);
+    top = wave_max_u32(top);
     if ((tid & 63) == 0) tops[tid >> 6] = top;
     __syncthreads();
     for (int i = 0; i < 16; ++i) top = tops[i] > top ? tops[i] : top;

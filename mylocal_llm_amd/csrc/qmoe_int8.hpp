@@ -118,9 +118,6 @@ __device__ __forceinline__ double int8_value(int acc, float s, float c) { return
 // the border of two codes gets the same code however many tokens share the step.
 __device__ __forceinline__ float int8_hidden(double g, double u) { return (float)(g / (1.0 + exp(-g)) * u); }
 
-// largest of the wave
-__device__ __forceinline__ uint32_t wave_top(uint32_t v) { return wave_max_u32(v); }
-
 // LDS operations of this workgroup's waves before and after; requests for memory stay in flight.
 __device__ __forceinline__ void meet_lds() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");

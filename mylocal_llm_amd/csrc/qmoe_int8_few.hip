@@ -1,16 +1,16 @@
 // Products of 8-bit codes for a few tokens: the weights are streamed once.
 //
 // A workgroup of eight waves owns RT tiles of 16 channels (of both matrices of a pair) and the whole of K;
-// wave w takes the w-th eighth of the 64-column steps (neighbouring ones: it uses the activation lines it fetches whole).  A step is one 1 KB request for each tile, already the A operand
-// of the matrix instruction, and one B operand for each 16 tokens; the eight partial sums meet in LDS once, as
-// integers, so the split changes no bit of the result.  What bounds it is the memory: an instruction multiplies
+// wave w takes the w-th eighth of the 64-column steps (neighbouring ones: it uses the activation lines it
+// fetches whole).  A step is one 1 KB request for each tile, already the A operand of the matrix instruction,
+// and one B operand for each 16 tokens; the eight partial sums meet in LDS once, as integers, so the split
+// changes no bit of the result.  What bounds it is the memory: an instruction multiplies
 // 1 KB of weights in 16 cycles where a CU receives 1 KB in about 100, so the idle token columns cost nothing and
 // 1..16 tokens take the same time.  Up to U requests a wave and tile are outstanding while the previous U are
 // multiplied: 64 - 128 KB a CU, beyond the 48 KB that 6 TB/s needs at 2 us.
 #include "qmoe_int8.hpp"
 
 namespace qmoe {
-
 
 struct Few8Args {
     const uint8_t *w, *w2;
@@ -26,10 +26,11 @@ struct Few8Args {
     int ydt;
 };
 
-// NX < 0: rows of codes at any address, NX = 0: at multiples of four bytes, NX > 0: every workgroup quantises the rows itself (they are few: up to NX pieces of 4096 columns of a token, eight
-// values a thread and piece, kept in registers between the search for the largest and the codes), into LDS rows
-// kp + 16 bytes apart: eight neighbouring tokens' 16-byte pieces then lie in eight different bank groups.  The rows are
-// requested before the first weights, so that waiting for them does not wait for the weights.
+// NX < 0   rows of codes at any address
+// NX = 0   at multiples of four bytes
+// NX > 0   every workgroup quantises the token itself: NX pieces of eight values a thread, kept in registers between the
+//          search for the largest and the codes.  They are requested before the first weights, so that waiting for them
+//          does not wait for the weights.
 template <int XDT, bool PAIR, int NX, int TT, int RT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Few8Args a) {
     constexpr bool FUSED = NX > 0, SHIFT = NX < 0;
@@ -88,7 +89,7 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Few8Args a) 
             uint32_t top = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) { const uint32_t b = abs_bits(v[p][j]); top = b > top ? b : top; }
-            top = wave_top(top);
+            top = wave_max_u32(top);
             if (lane == 0) tops[p * WAVES + wave] = top;
         }
         __syncthreads();

@@ -17,8 +17,7 @@ __global__ __launch_bounds__(64 * WN * WT) __attribute__((amdgpu_waves_per_eu(2)
                                                                  const Int8Product side_args, int side_n, int side_t) {
     constexpr int THREADS = 64 * WN * WT, NP = PAIR ? 2 : 1, NW = RT * NP;
     constexpr int ROWS = 16 * TT * WT, PIECES = KC / 16, KK = KC / 64, LOADS = ROWS * PIECES / THREADS;
-    // (four pieces a row: two rows are written by eight neighbouring lanes)
-    auto swap = [](int pc) { return KC == 64 ? 2 * (pc & 3) : pc & 7; };
+    auto swap = [](int pc) { return pc & 7; };
     static_assert(ROWS * PIECES % THREADS == 0 && LOADS > 0, "whole pieces a thread");
     __shared__ __align__(16) uint8_t lds[2 * ROWS * KC];
     __shared__ float srow[ROWS];
@@ -176,7 +175,9 @@ __global__ __launch_bounds__(64 * WN * WT) __attribute__((amdgpu_waves_per_eu(2)
             c[i][j] = ldg<float>(a.c + ch);
             if (PAIR) c2[i][j] = ldg<float>(a.c2 + ch);
         }
-    // 16-bit results in fp32: three roundings of 2^-24 in front of one of 2^-9 or 2^-12, a quarter of the instructions
+    // 16-bit results in fp32: three roundings of 2^-24 in front of one of 2^-9 or 2^-12, a quarter of the instructions.  Scales
+    // whose product would leave fp32's normal range take the 64-bit way at the end.
+    auto tame = [](float v) { return v == 0.0f || (fabsf(v) >= 0x1p-60f && fabsf(v) <= 0x1p60f); };
     auto value32 = [&](int i, int t, int j, float s) -> float {
         const float y = (float)acc[i * NP][t][j] * (s * (float)c[i][j]);
         if (!PAIR) return y;
@@ -196,6 +197,14 @@ __global__ __launch_bounds__(64 * WN * WT) __attribute__((amdgpu_waves_per_eu(2)
             }
         }
     };
+    bool plain = true;
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) plain = plain && tame((float)c[i][j]) && (!PAIR || tame((float)c2[i][j]));
+#pragma unroll
+    for (int t = 0; t < TT; ++t) plain = plain && tame(srow[(wt * TT + t) * 16 + col]);
+    plain = __all(plain);
     const bool whole = ((bn * WN + wn) * RT + RT) * 16 <= a.n && a.ldy % 4 == 0 && (uintptr_t)a.y % 16 == 0;
     if (whole && a.ydt == QMOE_DT_F32) {
 #pragma unroll
@@ -210,9 +219,9 @@ __global__ __launch_bounds__(64 * WN * WT) __attribute__((amdgpu_waves_per_eu(2)
                                                         value(i, t, 2, s, c[i][2], c2[i][2]), value(i, t, 3, s, c[i][3], c2[i][3])));
             }
         }
-    } else if (whole && a.ydt == QMOE_DT_BF16) {
+    } else if (whole && plain && a.ydt == QMOE_DT_BF16) {
         store16([](float v) -> uint32_t { return __builtin_bit_cast(uint16_t, (__bf16)v); });
-    } else if (whole) {
+    } else if (whole && plain) {
         store16([](float v) -> uint32_t { return __half_as_ushort(__float2half_rn(v)); });
     } else {
 #pragma unroll

@@ -60,7 +60,7 @@ __global__ __launch_bounds__(320) void int8_route_kernel(const void* __restrict_
                 if (i < 2048) v[j] = u[j];
             }
         }
-        top = wave_top(top);
+        top = wave_max_u32(top);
         if (lane == 0) tops[tid >> 6] = top;
     }
     __syncthreads();
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(256) void int8_hidden_rows_kernel(const Int8Rows ro
             if (!i0) v[j] = u[j];
         }
     }
-    top = wave_top(top);
+    top = wave_max_u32(top);
     if ((tid & 63) == 0) tops[tid >> 6] = top;
     __syncthreads();
 #pragma unroll

@@ -117,7 +117,7 @@ __global__ __launch_bounds__(64 * WAVES) void int8_front_kernel(const Front8Args
         uint32_t top = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) { const uint32_t b = abs_bits(w[j]); top = b > top ? b : top; }
-        if (wave_row) top = wave_top(top);
+        if (wave_row) top = wave_max_u32(top);
         if (gi < groups && (!wave_row || lane == 0)) atomicMax(&tops[over(gi, a.per_magic)], top);
     };
     auto turns = [&](auto&& f) {                   // every turn of eight values: the first ones from registers
@@ -398,7 +398,7 @@ __global__ __launch_bounds__(256) void int8_hidden_codes_kernel(const Back8Args 
     int8_load8<QMOE_DT_F32>(h, tid * 8 < wide ? tid * 8 : 0, wide - tid * 8, wide % 8 == 0, v);
     uint32_t top = 0;
     for (int i = tid; i < tiles; i += 256) { const uint32_t b = ldg<uint32_t>((sh ? a.in.sh_top : a.in.h_top) + at * tiles + i); top = b > top ? b : top; }
-    top = wave_top(top);
+    top = wave_max_u32(top);
     if ((tid & 63) == 0) tops[tid >> 6] = top;
     __syncthreads();
     for (int i = 0; i < 4; ++i) top = tops[i] > top ? tops[i] : top;
@@ -506,7 +506,7 @@ template <bool CODES> __global__ __launch_bounds__(BACK8_THREADS) void int8_back
             for (int p = 0; p < NX; ++p) {
                 if (n + p * BACK8_WAVES < all) {
                     const Turn c = turn(n + p * BACK8_WAVES);
-                    const RowScale rs(wave_top(part[p]));
+                    const RowScale rs(wave_max_u32(part[p]));
                     if (lane == 0 && c.i == 0) srow[(c.sh ? pairs : 0) + c.r] = rs.s;
                     const int i = c.i + lane * 8;
                     const u32x2_t q = int8_code8(v[p], rs);

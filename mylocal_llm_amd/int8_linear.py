@@ -2,8 +2,8 @@
 
 Both sides are int8: weights with a scale for each output channel, activations with a scale for each
 token, quantised on the way (``int8_quantize``) or given as codes.  The sum of code products is exact
-in int32, so a result is ``(sum q w) * s * c`` rounded once to the output type, whatever the number of
-tokens.  The reference keeps activations in floating point (mini_llm/ops/quantized_linear.py:272-400);
+in int32, so a result is ``(sum q w) * s * c`` to one rounding of the output type, whatever the number of
+tokens (16-bit results of many tokens are scaled in fp32, three roundings of 2^-24, before it).  The reference keeps activations in floating point (mini_llm/ops/quantized_linear.py:272-400);
 these operators stand beside ``quantized_linear`` / ``quantized_swiglu``, which take an ``Int8Weight``
 wherever they take a packed GGUF weight.
 """
@@ -16,6 +16,7 @@ from .quantized_linear import _TORCH_DTYPE_ID, DevicePackedGGUFWeight
 
 MAX_K = 131071            # 128 * 128 * K stays inside int32
 _INT8 = 3                 # QMOE_DT_INT8
+_MOST = 2 ** 31 - 1       # what the C entries' sizes hold
 
 
 def _call(device, function, *args):
@@ -61,6 +62,8 @@ def int8_quantize(x):
     if x.dtype not in _TORCH_DTYPE_ID:
         raise TypeError("Rows to quantise must be FP16, BF16, or FP32")
     k = x.shape[-1]
+    if max(k, x.numel() // k) > _MOST:
+        raise NotImplementedError(f"Rows to quantise: at most {_MOST} rows and columns")
     codes = torch.empty_like(x, dtype=torch.int8)
     scales = x.new_empty(x.shape[:-1], dtype=torch.float32)
     if x.numel():
@@ -82,6 +85,8 @@ def _tiles_of(codes, scales, dims, what):
     if not codes.is_contiguous() or not scales.is_contiguous():
         raise ValueError(f"{what} codes and scales must be contiguous")
     n, k = codes.shape[-2:]
+    if n > _MOST:
+        raise NotImplementedError(f"{what}: at most {_MOST} rows a matrix")
     if k > MAX_K:
         raise NotImplementedError(f"{what}: K beyond {MAX_K}, where an int32 sum could overflow")
     count = codes.shape[0] if dims == 3 else 1
@@ -150,6 +155,8 @@ def _activations(x, x_scales, k, device, out_dtype, what):
         raise ValueError("GPU input must be a contiguous tensor")
     if x.device != device:
         raise ValueError("all operands must be on the same device")
+    if x.numel() // k > _MOST:
+        raise NotImplementedError(f"{what}: at most {_MOST} rows")
     if out_dtype is not None and out_dtype not in _TORCH_DTYPE_ID:
         raise TypeError("out_dtype must be FP16, BF16, or FP32")
     if x.dtype == torch.int8:

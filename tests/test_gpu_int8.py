@@ -4,7 +4,8 @@ Tolerances (before any run): codes and scales are equal.  A product is an exact 
 bits, rounded to fp32 (2^-24) and then to its type (eps / 2, or half the smallest subnormal).  SwiGLU in fp32: g and
 u carry 2^-24 each, silu'(g) g / silu(g) is at most |g| + 1, and exp, the division and two products add a few units:
 (|g| + 8) 2^-24.  The step adds k weighted outputs (+ shared + residual), each rounded (k + 4 roundings of 2^-24 of the
-sum of magnitudes at most), and the admission gate's fp32 dot product.
+sum of magnitudes at most), and the admission gate's fp32 dot product.  Products of many tokens scale 16-bit results in
+fp32: the sum's conversion, s * c and their product round, 3 * 2^-24 instead of one, for g and u too.
 """
 import numpy as np
 import pytest
@@ -36,6 +37,11 @@ def close(got, want, rel32, extra=0.0):
     bound = np.abs(want) * (rel32 + half) * (1 + rel32) + extra * (1 + half) + info.smallest_normal * info.eps / 2
     bad = ~(np.abs(got - want) <= bound)
     assert not bad.any(), (int(bad.sum()), bad.size, float(np.nanmax(np.abs(got - want) / np.maximum(bound, 1e-300))))
+
+
+def front(dtype):
+    """Roundings of 2^-24 in front of the one to the output's type."""
+    return 1.01 if dtype == torch.float32 else 3.01
 
 
 def rows(t, k, seed, dtype=torch.float32, device="cuda"):
@@ -138,12 +144,48 @@ def test_linear_is_the_exact_sum_rounded_once(cuda, t, n, k, dtype):
     want = Q.product(q, s, *host(w))
     got = int8_linear(x, weight)
     assert got.dtype == dtype and got.shape == (t, n)
-    close(got, want, 1.01 * U)
+    close(got, want, front(dtype) * U)
     codes, scales = int8_quantize(x)
     again = int8_linear(codes, weight, x_scales=scales, out_dtype=dtype)
     assert torch.equal(again, got)           # the same integers, the same scales
     if dtype != torch.float32:
         close(int8_linear(x, weight, out_dtype=torch.float32), want, 1.01 * U)
+
+
+# sizes behind each of the tiles for many tokens, whole and with rests on every side; K from one column to many chunks
+TILED = [(950, 3590, 1), (960, 3584, 200), (1800, 4096, 64), (1790, 4090, 321), (4096, 4096, 72), (4001, 4085, 130), (700, 704, 1100), (690, 1000, 513)]
+
+
+@pytest.mark.parametrize("t,n,k", TILED)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_tiles_of_many_tokens(cuda, t, n, k, dtype):
+    announce("int8 tiles", t, n, k, dtype)
+    x, g, u = rows(t, k, t + n, dtype), matrix(n, k, n + k), matrix(n, k, n + k + 1)
+    g[1].mul_(20.0 / k ** 0.5)
+    gate, up = Int8Weight(*g), Int8Weight(*u)
+    q, s = Q.quantize(as_np(x))
+    gv, uv = Q.product(q, s, *host(g)), Q.product(q, s, *host(u))
+    got = int8_linear(x, gate)
+    close(got, gv, front(dtype) * U)
+    close(int8_swiglu(x, gate, up), Q.swish(gv, uv), (front(dtype) * np.abs(gv) + 12) * U)
+    codes, scales = int8_quantize(x)
+    assert torch.equal(int8_linear(codes, gate, x_scales=scales, out_dtype=dtype), got)
+    some = torch.arange(0, t, 97, device=cuda)
+    few = int8_linear(x[some].contiguous(), gate, out_dtype=torch.float32)
+    assert torch.equal(int8_linear(x, gate, out_dtype=torch.float32)[some], few)      # one formula on every path
+
+
+@pytest.mark.parametrize("t,n,k", [(1, 700, 200), (20, 700, 200), (100, 704, 200), (720, 704, 200), (720, 1001, 64)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_scales_far_from_one(cuda, t, n, k, dtype):
+    """s * c beyond fp32's normal range on either side, results inside it.  (extra: half of fp32's smallest subnormal)"""
+    announce("int8 scales", t, n, k, dtype)
+    x, (codes, scales) = rows(t, k, t), matrix(n, k, n)
+    x = (x * torch.tensor([1e-39, 1e-30, 1e-10, 1.0, 1e10, 1e28], device=cuda)[torch.arange(t, device=cuda) % 6][:, None]).to(dtype)
+    scales = scales * torch.tensor([1e-8, 1.0, 1e4], device=cuda)[torch.arange(n, device=cuda) % 3]
+    scales[5::50] = 0.0
+    q, s = Q.quantize(as_np(x))
+    close(int8_linear(x, Int8Weight(codes, scales)), Q.product(q, s, codes.cpu().numpy(), scales.cpu().numpy()), front(dtype) * U, 2.0 ** -150)
 
 
 @pytest.mark.parametrize("t", [1, 5, 16, 40, 130])
@@ -239,7 +281,7 @@ def test_swiglu(cuda, t, f, k, dtype):
     want = Q.swish(gv, uv)
     got = int8_swiglu(x, Int8Weight(*g), Int8Weight(*u))
     assert got.dtype == dtype
-    close(got, want, (np.abs(gv) + 8) * U)
+    close(got, want, (front(dtype) * np.abs(gv) + 12) * U)
     codes, scales = int8_quantize(x)
     assert torch.equal(int8_swiglu(codes, Int8Weight(*g), Int8Weight(*u), x_scales=scales, out_dtype=dtype), got)
 
