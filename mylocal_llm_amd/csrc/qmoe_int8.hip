@@ -167,7 +167,7 @@ static int dense(const char* who, bool pair, const void* w, const float* c, cons
     a.n = n; a.kp = (int)int8_cols64(k); a.tokens = tokens; a.y = y; a.ydt = ydt; a.ldy = n; a.ld = int8_cols256(k);
     a.q = (const uint8_t*)x; a.s = xs;
     if (xdt != QMOE_DT_I8 && int8_few_fuses(tokens, k)) return int8_few_launch(a, pair, x, xdt, k, st);
-    const bool few = int8_few_takes(n, tokens);
+    const bool few = int8_few_takes(n, tokens, pair);
     if (xdt != QMOE_DT_I8) {
         uint8_t* const q = (uint8_t*)workspace;
         float* const s = (float*)(q + round256((size_t)tokens * a.ld));
@@ -217,7 +217,7 @@ int qmoe_int8_tiles(const void* codes, int64_t matrices, int n, int k, void* til
 
 size_t qmoe_int8_workspace_bytes(int n, int k, int tokens, int x_dtype) {
     if (n < 1 || k < 1 || tokens < 1) return 0;
-    if (x_dtype == QMOE_DT_INT8 ? int8_few_takes(n, tokens) : int8_few_fuses(tokens, k)) return 0;
+    if (x_dtype == QMOE_DT_INT8 ? int8_few_takes(n, tokens, false) : int8_few_fuses(tokens, k)) return 0;
     return round256((size_t)tokens * (size_t)int8_cols256(k)) + round256((size_t)tokens * 4);
 }
 

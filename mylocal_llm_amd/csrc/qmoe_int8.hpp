@@ -132,7 +132,7 @@ int int8_quantize_launch(const void* x, int dt, int64_t rows, int k, uint8_t* co
 // Whether a product of these rows quantises them in its own workgroups, whether it is one of few tokens, and its launch (x: rows
 // to quantise, NULL: p.q holds codes, any alignment).
 bool int8_few_fuses(int tokens, int k);
-bool int8_few_takes(int n, int tokens);
+bool int8_few_takes(int n, int tokens, bool pair);
 struct Int8Product;
 int int8_few_launch(const Int8Product& p, bool pair, const void* x, int xdt, int k, hipStream_t s);
 int int8_gemm_launch(const Int8Product& a, bool pair, hipStream_t s);

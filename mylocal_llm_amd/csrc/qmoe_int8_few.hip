@@ -222,20 +222,23 @@ static int few8_as(const Few8Args& a, hipStream_t s) {
 static int few8_pieces(int k) { return (k + 4095) / 4096; }
 bool int8_few_fuses(int tokens, int k) { return tokens == 1 && few8_pieces(k) <= 4; }
 
-// Up to 64 tokens, and more where 64 x 64 tiles would leave most of the chip without a workgroup.
-bool int8_few_takes(int n, int tokens) { return tokens <= 64 || ((n + 63ll) / 64) * ((tokens + 63ll) / 64) < 96; }
+// Up to 16 tokens, and more where blocks of 16 channels x 32 tokens are few: there the waves' cut of K beats tiles that walk K as
+// a whole (us, cold; this kernel / tiles: 17 x 4096 x 4096 7.5 / 8.2, 32 x 4096 x 4096 8.8 / 8.4, 32 x 4096 x 14336 23.8 / 20.3,
+// 64 x 4096 x 4096 12.8 / 8.7; pairs 32 x 4096 x 4096 10.6 / 12.2, 128 x 1024 x 4096 8.6 / 11.0, 128 x 4096 x 4096 27 / 15).
+bool int8_few_takes(int n, int tokens, bool pair) {
+    const int64_t blocks = (n + 15ll) / 16 * ((tokens + 31ll) / 32);
+    return tokens <= 16 || blocks <= 192 || (blocks <= 256 && (pair || tokens <= 24));
+}
 
 template <int XDT, bool PAIR, int RT> static int few8_fused(const Few8Args& a, int waves, hipStream_t s) {
     if (waves == 16) return few8_pieces(a.k) <= 2 ? few8_as<XDT, PAIR, 1, 1, 1, 16>(a, s) : few8_as<XDT, PAIR, 2, 1, 1, 16>(a, s);
     return few8_pieces(a.k) == 1 ? few8_as<XDT, PAIR, 1, 1, RT, 8>(a, s) : few8_as<XDT, PAIR, 4, 1, RT, 8>(a, s);
 }
-template <bool PAIR> static int few8_codes(const Few8Args& a, int rt, int waves, hipStream_t s) {
+template <bool PAIR> static int few8_codes(const Few8Args& a, int rt, hipStream_t s) {
     // rows at odd addresses: whole dwords and a shift (as they are, 77 x 1001 x 1234 takes 10.9 us, so 7.6, at multiples of four 5.4)
     if (((uintptr_t)a.q | (uintptr_t)a.ld) % 4) return a.tokens <= 16 ? few8_as<0, PAIR, -1, 1, 1, 8>(a, s) : few8_as<0, PAIR, -1, 2, 1, 8>(a, s);
-    if (a.tokens > 64) return few8_as<0, PAIR, 0, 2, 1, 8>(a, s);      // blocks of 32 tokens
-    if (a.tokens <= 16) return waves == 16 ? few8_as<0, PAIR, 0, 1, 1, 16>(a, s) : rt == 1 ? few8_as<0, PAIR, 0, 1, 1, 8>(a, s) : few8_as<0, PAIR, 0, 1, 2, 8>(a, s);
-    if (a.tokens <= 32) return rt == 1 ? few8_as<0, PAIR, 0, 2, 1, 8>(a, s) : few8_as<0, PAIR, 0, 2, 2, 8>(a, s);
-    return rt == 1 ? few8_as<0, PAIR, 0, 4, 1, 8>(a, s) : rt == 2 || PAIR ? few8_as<0, PAIR, 0, 4, 2, 8>(a, s) : few8_as<0, PAIR, 0, 4, PAIR ? 2 : 4, 8>(a, s);
+    if (a.tokens > 16) return few8_as<0, PAIR, 0, 2, 1, 8>(a, s);      // blocks of 32 tokens
+    return rt == 1 ? few8_as<0, PAIR, 0, 1, 1, 8>(a, s) : few8_as<0, PAIR, 0, 1, 2, 8>(a, s);
 }
 
 int int8_few_launch(const Int8Product& p, bool pair, const void* x, int xdt, int k, hipStream_t s) {
@@ -244,13 +247,13 @@ int int8_few_launch(const Int8Product& p, bool pair, const void* x, int xdt, int
     a.q = p.q; a.ld = p.ld; a.s = p.s; a.tokens = p.tokens; a.y = p.y; a.ydt = p.ydt;
     // Two tiles a workgroup once they still make two workgroups a CU: fewer prologues and half the activation reads for the
     // same weights (8192 x 4096 even, 14336 x 4096 13.4 -> 12.2 us, 151936 x 2048 67.5 -> 49.8 us at one token; 4096 x 4096
-    // 5.6 -> 6.8 us); four for more than 32 tokens and 768 tiles (64 x 14336 x 4096: 44.3 / 28.8 / 21.5 us with 1 / 2 / 4).
+    // 5.6 -> 6.8 us).
     // Sixteen waves where one token's row is long and the workgroups are few (4096 x 14336: 15.9 -> 14.4 us).
     const int tiles = (p.n + 15) / 16;
-    const int rt = tiles < 512 ? 1 : tiles >= 768 && p.tokens > 32 ? 4 : 2;
+    const int rt = tiles < 512 ? 1 : 2;
     const int waves = x && k > 4096 && tiles < 512 ? 16 : 8;
     a.k = x ? k : (int)(p.ld < p.kp ? k : p.kp);
-    if (!x) return pair ? few8_codes<true>(a, rt, waves, s) : few8_codes<false>(a, rt, waves, s);
+    if (!x) return pair ? few8_codes<true>(a, rt, s) : few8_codes<false>(a, rt, s);
     a.x = x;
     a.fast = (uintptr_t)x % 16 == 0 && k % 8 == 0;
 #define QMOE_FUSED(DT) (pair ? few8_fused<DT, true, 1>(a, waves, s) : rt == 1 ? few8_fused<DT, false, 1>(a, waves, s) : few8_fused<DT, false, 2>(a, waves, s))

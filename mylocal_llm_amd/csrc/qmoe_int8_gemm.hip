@@ -12,7 +12,8 @@
 
 namespace qmoe {
 
-template <bool PAIR, bool HIDDEN, bool PLAN, int WN, int WT, int RT, int TT, int KC, int R>
+// R: steps of 64 columns that the weights' requests run ahead; XR: chunks that the activations' requests run ahead.
+template <bool PAIR, bool HIDDEN, bool PLAN, int WN, int WT, int RT, int TT, int KC, int R, int XR>
 __global__ __launch_bounds__(64 * WN * WT) __attribute__((amdgpu_waves_per_eu(2))) void int8_gemm_kernel(const Int8Product main_args, int n_blocks, int t_blocks,
                                                                  const Int8Product side_args, int side_n, int side_t) {
     constexpr int THREADS = 64 * WN * WT, NP = PAIR ? 2 : 1, NW = RT * NP;
@@ -79,14 +80,18 @@ __global__ __launch_bounds__(64 * WN * WT) __attribute__((amdgpu_waves_per_eu(2)
         const int pos = first + (i < count ? i : 0);
         srow[i] = a.s[PLAN && a.row_of ? a.row_of[pos] : pos];
     }
-    i32x4_t xr[LOADS], wr[R][NW];
-    auto request_x = [&](int chunk) {
+    constexpr int ROUND = R / KK > 2 ? R / KK : 2;       // chunks after which rings and buffers are back where they were
+    static_assert(ROUND % 2 == 0 && ROUND * KK % R == 0 && ROUND % XR == 0, "a round turns all rings whole");
+    const int end = chunks - 1;
+    i32x4_t xr[XR][LOADS], wr[R][NW];
+    auto request_x = [&](int chunk, i32x4_t (&x)[LOADS]) {
+        const int c = chunk < end ? chunk : end;
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) xr[i] = ldg_i32x4(x0 + (xp[i] + chunk * KC));
+        for (int i = 0; i < LOADS; ++i) x[i] = ldg_i32x4(x0 + (xp[i] + c * KC));
     };
-    auto keep_x = [&](int buffer) {
+    auto keep_x = [&](int buffer, const i32x4_t (&x)[LOADS]) {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) *(i32x4_t*)(lds + buffer * (ROWS * KC) + slot[i]) = xr[i];
+        for (int i = 0; i < LOADS; ++i) *(i32x4_t*)(lds + buffer * (ROWS * KC) + slot[i]) = x[i];
     };
     // (steps behind the last repeat it: they meet activations of zero, or nothing; what is in flight never depends on a
     // condition)
@@ -116,11 +121,10 @@ __global__ __launch_bounds__(64 * WN * WT) __attribute__((amdgpu_waves_per_eu(2)
     };
     // A chunk in halves of a step: while one half is multiplied the next half's operands are read, and the last half of a
     // chunk is multiplied behind the meeting that opens the next one.  A step's weights are requested again into the
-    // registers they leave, R steps ahead; activations are requested two chunks ahead of their use.
-    const int end = chunks - 1;
+    // registers they leave, R steps ahead; activations are requested XR + 1 chunks ahead of their use.
     auto turn = [&](int c, int h) {
-        keep_x((h + 1) & 1);
-        request_x(c + 2 < end ? c + 2 : end);
+        keep_x((h + 1) & 1, xr[(h + 1) % XR]);
+        request_x(c + 1 + XR, xr[(h + 1) % XR]);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < 2 * KK; ++j) {
@@ -138,11 +142,11 @@ __global__ __launch_bounds__(64 * WN * WT) __attribute__((amdgpu_waves_per_eu(2)
             __builtin_amdgcn_sched_barrier(0);     // (the scheduler would gather the requests behind the products)
         }
     };
-    constexpr int ROUND = R / KK > 2 ? R / KK : 2;       // chunks after which ring and buffers are back where they were
-    static_assert(ROUND % 2 == 0 && ROUND * KK % R == 0, "a round turns both rings whole");
-    request_x(0);
-    keep_x(0);
-    request_x(1 < end ? 1 : end);
+    request_x(0, xr[0]);
+    keep_x(0, xr[0]);
+#pragma unroll
+    for (int i = 1; i <= XR; ++i) request_x(i, xr[i % XR]);
+    __builtin_amdgcn_sched_barrier(0);      // (requests come back in order, and the loop waits for these first)
 #pragma unroll
     for (int r = 0; r < R; ++r) request_w(r, wr[r]);
     meet_lds();
@@ -238,13 +242,13 @@ __global__ __launch_bounds__(64 * WN * WT) __attribute__((amdgpu_waves_per_eu(2)
     }
 }
 
-template <bool PAIR, bool HIDDEN, bool PLAN, int WN, int WT, int RT, int TT, int KC, int R>
+template <bool PAIR, bool HIDDEN, bool PLAN, int WN, int WT, int RT, int TT, int KC, int R, int XR>
 static int gemm8_as(const Int8Product& a, int chunks, hipStream_t s, const Int8Product* side = nullptr) {
     const int nb = (a.n + 16 * WN * RT - 1) / (16 * WN * RT), tb = PLAN ? (chunks + 31) / 32 * 32 : (a.tokens + 16 * WT * TT - 1) / (16 * WT * TT);
     const int sn = side ? (side->n + 16 * WN * RT - 1) / (16 * WN * RT) : 0, st = side ? (side->tokens + 16 * WT * TT - 1) / (16 * WT * TT) : 0;
     if (((int64_t)nb * tb + (int64_t)sn * st) * (64 * WN * WT) > 0xFFFFFFFFll)      // (a launch's threads are counted in 32 bits)
         return fail(QMOE_EUNSUPPORTED, "int8 product: %d x %d blocks exceed a launch; split the tokens", nb, tb);
-    hipLaunchKernelGGL((int8_gemm_kernel<PAIR, HIDDEN, PLAN, WN, WT, RT, TT, KC, R>), dim3(nb * tb + sn * st), dim3(64 * WN * WT), 0, s, a, nb, PLAN ? chunks : tb,
+    hipLaunchKernelGGL((int8_gemm_kernel<PAIR, HIDDEN, PLAN, WN, WT, RT, TT, KC, R, XR>), dim3(nb * tb + sn * st), dim3(64 * WN * WT), 0, s, a, nb, PLAN ? chunks : tb,
                        side ? *side : a, sn, st);
     return check_launch("int8 product");
 }
@@ -257,13 +261,13 @@ int int8_plan_rows(int64_t assignments, int n_experts) {
 // side: NULL, or a dense product of the same kind (pair with the hidden activation, or plain) that rides in front.
 int int8_plan_launch(const Int8Product& a, bool pair, int rows, int max_chunks, const Int8Product* side, hipStream_t s) {
     if (pair) {
-        if (rows == 32) return gemm8_as<true, true, true, 4, 1, 1, 2, 256, 8>(a, max_chunks, s, side);
-        if (rows == 64) return gemm8_as<true, true, true, 4, 1, 1, 4, 256, 8>(a, max_chunks, s, side);
-        return gemm8_as<true, true, true, 4, 1, 2, 8, 128, 4>(a, max_chunks, s, side);
+        if (rows == 32) return gemm8_as<true, true, true, 4, 1, 1, 2, 256, 8, 2>(a, max_chunks, s, side);
+        if (rows == 64) return gemm8_as<true, true, true, 4, 1, 1, 4, 256, 8, 1>(a, max_chunks, s, side);
+        return gemm8_as<true, true, true, 4, 1, 2, 8, 128, 4, 1>(a, max_chunks, s, side);
     }
-    if (rows == 32) return gemm8_as<false, false, true, 4, 1, 2, 2, 256, 4>(a, max_chunks, s, side);
-    if (rows == 64) return gemm8_as<false, false, true, 4, 1, 2, 4, 256, 8>(a, max_chunks, s, side);
-    return gemm8_as<false, false, true, 4, 1, 4, 8, 128, 4>(a, max_chunks, s, side);
+    if (rows == 32) return gemm8_as<false, false, true, 4, 1, 2, 2, 256, 4, 2>(a, max_chunks, s, side);
+    if (rows == 64) return gemm8_as<false, false, true, 4, 1, 2, 4, 256, 8, 1>(a, max_chunks, s, side);
+    return gemm8_as<false, false, true, 4, 1, 4, 8, 128, 4, 1>(a, max_chunks, s, side);
 }
 
 // The largest tile that still gives nearly every CU a workgroup (us from codes; 256 x 256 of eight waves / 256 channels x
@@ -280,12 +284,17 @@ int int8_gemm_launch(const Int8Product& a, bool pair, hipStream_t s) {
     const int wide = pair ? 128 : 256;
     const int64_t large = blocks(wide, 256), rounds = (large + CUS - 1) / CUS * CUS;
     if (large >= ENOUGH && large * 20 >= rounds * 19)
-        return pair ? gemm8_as<true, false, false, 4, 2, 2, 8, 128, 4>(a, 0, s) : gemm8_as<false, false, false, 4, 2, 4, 8, 128, 4>(a, 0, s);
+        return pair ? gemm8_as<true, false, false, 4, 2, 2, 8, 128, 4, 1>(a, 0, s) : gemm8_as<false, false, false, 4, 2, 4, 8, 128, 4, 1>(a, 0, s);
     if (blocks(wide, 128) >= ENOUGH)
-        return pair ? gemm8_as<true, false, false, 4, 1, 2, 8, 128, 4>(a, 0, s) : gemm8_as<false, false, false, 4, 1, 4, 8, 128, 4>(a, 0, s);
+        return pair ? gemm8_as<true, false, false, 4, 1, 2, 8, 128, 4, 1>(a, 0, s) : gemm8_as<false, false, false, 4, 1, 4, 8, 128, 4, 1>(a, 0, s);
     if (blocks(wide, 64) >= ENOUGH)
-        return pair ? gemm8_as<true, false, false, 4, 1, 2, 4, 128, 4>(a, 0, s) : gemm8_as<false, false, false, 4, 1, 4, 4, 128, 4>(a, 0, s);
-    return pair ? gemm8_as<true, false, false, 4, 1, 1, 2, 256, 8>(a, 0, s) : gemm8_as<false, false, false, 4, 1, 1, 4, 256, 8>(a, 0, s);
+        return pair ? gemm8_as<true, false, false, 4, 1, 2, 4, 128, 4, 1>(a, 0, s) : gemm8_as<false, false, false, 4, 1, 4, 4, 128, 4, 1>(a, 0, s);
+    if (!pair && blocks(128, 64) >= ENOUGH) return gemm8_as<false, false, false, 4, 1, 2, 4, 256, 8, 1>(a, 0, s);
+    if (blocks(64, 64) >= ENOUGH)
+        return pair ? gemm8_as<true, false, false, 4, 1, 1, 4, 256, 8, 2>(a, 0, s) : gemm8_as<false, false, false, 4, 1, 1, 4, 256, 8, 1>(a, 0, s);
+    if (blocks(64, 32) >= 192)
+        return pair ? gemm8_as<true, false, false, 4, 1, 1, 2, 256, 8, 2>(a, 0, s) : gemm8_as<false, false, false, 4, 1, 1, 2, 256, 8, 2>(a, 0, s);
+    return pair ? gemm8_as<true, false, false, 2, 1, 1, 2, 256, 16, 4>(a, 0, s) : gemm8_as<false, false, false, 2, 1, 1, 2, 256, 16, 4>(a, 0, s);
 }
 
 }  // namespace qmoe
