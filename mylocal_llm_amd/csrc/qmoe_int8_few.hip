@@ -7,7 +7,11 @@
 // changes no bit of the result.  What bounds it is the memory: an instruction multiplies
 // 1 KB of weights in 16 cycles where a CU receives 1 KB in about 100, so the idle token columns cost nothing and
 // 1..16 tokens take the same time.  Up to U requests a wave and tile are outstanding while the previous U are
-// multiplied: 64 - 128 KB a CU, beyond the 48 KB that 6 TB/s needs at 2 us.
+// multiplied: four.  (Eight, with one tile: 16 x 4096 x 4096 7.3 instead of 6.7 us, 1 x 512 x 512 2.6 instead of 2.2,
+// 77 x 1001 x 1234 7.8 instead of 5.4: a short wave requests what it does not need.  Two, with two tiles at one token:
+// 1 x 151936 x 2048 54 instead of 49 us.)
+// From codes in memory, us: 1 x 4096 x 4096 5.5 (16.8 MB: 3.1 TB/s, the launch and its end are half of it),
+// 1 x 14336 x 4096 12.1 (4.9 TB/s), 16 x 14336 x 4096 13.6, 1 x 151936 x 2048 49 (6.3 TB/s).
 #include "qmoe_int8.hpp"
 
 namespace qmoe {
@@ -35,7 +39,7 @@ template <int XDT, bool PAIR, int NX, int TT, int RT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Few8Args a) {
     constexpr bool FUSED = NX > 0, SHIFT = NX < 0;
     constexpr int THREADS = 64 * WAVES;
-    constexpr int NP = PAIR ? 2 : 1, NW = RT * NP, U = NW >= 8 ? 1 : 8 / NW;
+    constexpr int NP = PAIR ? 2 : 1, NW = RT * NP, U = NW == 1 ? 4 : (TT == 1 ? 8 : 4) / NW;
     extern __shared__ uint8_t lds[];       // [codes] and, over them at the end, [waves][NW][TT][64] partial sums
     __shared__ uint32_t tops[FUSED ? NX * WAVES : 1];
     __shared__ float srow[16 * TT];
@@ -235,7 +239,7 @@ template <int XDT, bool PAIR, int RT> static int few8_fused(const Few8Args& a, i
     return few8_pieces(a.k) == 1 ? few8_as<XDT, PAIR, 1, 1, RT, 8>(a, s) : few8_as<XDT, PAIR, 4, 1, RT, 8>(a, s);
 }
 template <bool PAIR> static int few8_codes(const Few8Args& a, int rt, hipStream_t s) {
-    // rows at odd addresses: whole dwords and a shift (as they are, 77 x 1001 x 1234 takes 10.9 us, so 7.6, at multiples of four 5.4)
+    // rows at odd addresses: whole dwords and a shift (77 x 1001 x 1234: 5.5 us, its neighbour of 1236 columns, at multiples of four, 4.4)
     if (((uintptr_t)a.q | (uintptr_t)a.ld) % 4) return a.tokens <= 16 ? few8_as<0, PAIR, -1, 1, 1, 8>(a, s) : few8_as<0, PAIR, -1, 2, 1, 8>(a, s);
     if (a.tokens > 16) return few8_as<0, PAIR, 0, 2, 1, 8>(a, s);      // blocks of 32 tokens
     return rt == 1 ? few8_as<0, PAIR, 0, 1, 1, 8>(a, s) : few8_as<0, PAIR, 0, 1, 2, 8>(a, s);
