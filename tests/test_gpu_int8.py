@@ -65,7 +65,8 @@ def host(pair):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("t,k", [(1, 1), (1, 4096), (3, 7), (5, 64), (2, 63), (4, 65), (333, 1999), (7, 2048), (6, 2056), (9, 8192),
-                                 (2, 16384), (3, 14336), (1, 40000), (2, 131075), (1000, 2), (17, 516)])
+                                 (2, 16384), (3, 14336), (1, 40000), (2, 131075), (1000, 2), (17, 516),
+                                 (3, 32768), (2, 32776), (3, 65536), (2, 65544), (2, 20001), (2, 40001), (1030, 1024), (1024, 1031), (1100, 4104)])
 def test_codes_and_scales_are_the_definition(cuda, dtype, t, k):
     announce("quantise", dtype, t, k)
     x = rows(t, k, 1000 * t + k, dtype)
