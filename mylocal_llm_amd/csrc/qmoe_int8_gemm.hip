@@ -253,10 +253,12 @@ static int gemm8_as(const Int8Product& a, int chunks, hipStream_t s, const Int8P
     return check_launch("int8 product");
 }
 
-// A chunk of a plan holds up to `rows` sorted positions of one expert: 32, 64 or 128.
+// A chunk of a plan holds up to `rows` sorted positions of one expert: 32, 64 or 128, by the average (us of a whole step with
+// 32 / 64 / 128; 64 experts of width 1024, 128 of 512, 2048 columns): average 20 105 / 107 / 106 and 108 / 110 / 114, average 40
+// 133 / 117 / 116 and 138 / 125 / 129, average 90 190 / 168 / 142 and 208 / 183 / 171, average 256 399 / 315 / 271 and 490 / 405 / 352.
 int int8_plan_rows(int64_t assignments, int n_experts) {
     const int64_t average = assignments / n_experts;
-    return average <= 24 ? 32 : average <= 96 ? 64 : 128;
+    return average < 28 ? 32 : average <= 72 ? 64 : 128;
 }
 // side: NULL, or a dense product of the same kind (pair with the hidden activation, or plain) that rides in front.
 int int8_plan_launch(const Int8Product& a, bool pair, int rows, int max_chunks, const Int8Product* side, hipStream_t s) {
@@ -271,11 +273,14 @@ int int8_plan_launch(const Int8Product& a, bool pair, int rows, int max_chunks, 
 }
 
 // The largest tile that still gives nearly every CU a workgroup (us from codes; 256 x 256 of eight waves / 256 channels x
-// 128 tokens of four, two workgroups a CU / 256 x 64 / 64 x 64): 4096 tokens x 4096 x 14336 184 / 184 / 220 / 351,
-// 4096 x 14336 x 4096 225 / 213 / 268 / 380, 512 x 14336 x 4096 49 / 33 / 36 / 48, 1024 x 4096 x 4096 47 / 30 / 21 / 30,
-// 128 x 4096 x 4096 42 / 29 / 17 / 10.
+// 128 tokens of four, two workgroups a CU / 256 x 64 / 128 x 64 / 64 x 64 / 64 x 32 / 32 x 32): 4096 tokens x 4096 x 14336
+// 184 / 184 / 220 / - / 351, 4096 x 14336 x 4096 225 / 213 / 268 / - / 380, 512 x 14336 x 4096 49 / 33 / 36 / - / 48,
+// 1024 x 4096 x 4096 47 / 30 / 22 / 25 / 29, 128 x 14336 x 4096 - / - / 29 / 20 / 22 / 28, 512 x 2048 x 2048 - / - / 12 / 9.2 / 7.5 /
+// 7.7, 128 x 4096 x 4096 - / - / 18 / 13 / 12.4 / 10.0 / 12.2, 64 x 4096 x 14336 - / - / - / - / 35 / 27 / 20.
 // One workgroup a CU loses what the last round leaves empty, and nothing hides its start and its end: the largest tile is
 // taken where the rounds come out nearly even.
+// What bounds it: large sizes the matrix instructions and what feeds them (4096 x 4096 x 14336 2.8 POP/s, of 4.8 that the
+// instruction alone reaches), small ones the way from one chunk to the next, 0.2 - 0.4 us of meeting and latencies.
 int int8_gemm_launch(const Int8Product& a, bool pair, hipStream_t s) {
     auto blocks = [&](int channels, int tokens) {
         return (int64_t)((a.n + channels - 1) / channels) * ((a.tokens + tokens - 1) / tokens);

@@ -326,7 +326,8 @@ CASES = [  # tokens, experts, top_k, d_model, d_ff, d_shared
     (4, 32, 2, 192, 1536, 64), (5, 60, 4, 128, 704, 100), (9, 512, 10, 256, 64, 0), (15, 5, 5, 330, 130, 17), (16, 64, 6, 512, 256, 512),
     (16, 2, 1, 64, 2048, 0), (17, 16, 4, 256, 256, 256), (33, 9, 2, 130, 70, 0), (64, 40, 8, 256, 100, 128), (100, 3, 3, 77, 91, 13), (200, 64, 2, 320, 192, 0),
     (1, 8, 2, 4096, 300, 0), (7, 8, 2, 300, 4096, 0), (2, 4, 2, 8200, 80, 16),
-    (16, 12, 2, 8128, 1500, 0), (17, 6, 2, 8128, 100, 40), (64, 8, 4, 192, 160, 96), (40, 2, 1, 64, 300, 0), (300, 3, 2, 128, 130, 50)]
+    (16, 12, 2, 8128, 1500, 0), (17, 6, 2, 8128, 100, 40), (64, 8, 4, 192, 160, 96), (40, 2, 1, 64, 300, 0), (300, 3, 2, 128, 130, 50), (70, 2, 1, 200, 97, 0),
+    (120, 4, 1, 130, 70, 33), (220, 6, 2, 300, 190, 100), (400, 2, 1, 260, 65, 0)]
 
 
 @pytest.mark.parametrize("t,e,k,d,f,fs", CASES)
