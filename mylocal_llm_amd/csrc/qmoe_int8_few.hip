@@ -40,22 +40,20 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Few8Args a) 
     constexpr bool FUSED = NX > 0, SHIFT = NX < 0;
     constexpr int THREADS = 64 * WAVES;
     constexpr int NP = PAIR ? 2 : 1, NW = RT * NP, U = NW == 1 ? 4 : (TT == 1 ? 8 : 4) / NW;
-    extern __shared__ uint8_t lds[];       // [codes] and, over them at the end, [waves][NW][TT][64] partial sums
-    __shared__ uint32_t tops[FUSED ? NX * WAVES : 1];
+    extern __shared__ __align__(16) uint8_t lds[];       // [codes] and, over them at the end, [waves][NW][TT][64] partial sums
+    __shared__ uint32_t tops[WAVES];
     __shared__ float srow[16 * TT];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
     const int row_tiles = (a.n + 15) / 16;
     const int first = FUSED ? 0 : (int)blockIdx.y * 16 * TT, tokens = a.tokens - first < 16 * TT ? a.tokens - first : 16 * TT;
 
-    constexpr int PIECE = THREADS * 8;
-    const int per = (a.k + PIECE - 1) / PIECE;     // pieces of a token
     float v[FUSED ? NX : 1][8];
     if (FUSED) {
 #pragma unroll
         for (int p = 0; p < NX; ++p) {
-            const int t = p / per, i = (p % per) * PIECE + tid * 8, left = t < tokens ? a.k - i : 0;
-            int8_load8<XDT>(a.x, left > 0 ? (size_t)t * a.k + i : 0, left, a.fast, v[p]);
+            const int i = (p * THREADS + tid) * 8;
+            int8_load8<XDT>(a.x, i < a.k ? i : 0, a.k - i, a.fast, v[p]);
         }
     }
 
@@ -82,30 +80,27 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Few8Args a) 
     };
     request(0);
 
-    const int stride = a.kp + 16;
     const uint8_t* qp[TT];
     uint32_t shift[TT];
 #pragma unroll
     for (int t = 0; t < TT; ++t) shift[t] = 0;
     if (FUSED) {
+        uint32_t top = 0;
 #pragma unroll
-        for (int p = 0; p < NX; ++p) {
-            uint32_t top = 0;
+        for (int p = 0; p < NX; ++p)
 #pragma unroll
             for (int j = 0; j < 8; ++j) { const uint32_t b = abs_bits(v[p][j]); top = b > top ? b : top; }
-            top = wave_max_u32(top);
-            if (lane == 0) tops[p * WAVES + wave] = top;
-        }
+        top = wave_max_u32(top);
+        if (lane == 0) tops[wave] = top;
         __syncthreads();
 #pragma unroll
+        for (int j = 0; j < WAVES; ++j) top = tops[j] > top ? tops[j] : top;
+        const RowScale rs(top);
+        if (tid == 0) srow[0] = rs.s;
+#pragma unroll
         for (int p = 0; p < NX; ++p) {
-            const int t = p / per, i = (p % per) * PIECE + tid * 8;
-            if (t >= tokens) break;
-            uint32_t top = 0;
-            for (int j = t * per * WAVES; j < (t + 1) * per * WAVES; ++j) top = tops[j] > top ? tops[j] : top;
-            const RowScale rs(top);
-            if (tid == 0) srow[t] = rs.s;
-            if (i < a.kp) *(u32x2_t*)(lds + t * stride + i) = int8_code8(v[p], rs);
+            const int i = (p * THREADS + tid) * 8;
+            if (i < a.kp) *(u32x2_t*)(lds + i) = int8_code8(v[p], rs);
         }
         __syncthreads();
     } else {
@@ -143,7 +138,7 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Few8Args a) 
         }
     }
     const int chunks = hi > lo ? (hi - lo + U - 1) / U : 0;
-    const uint8_t* const mine = lds + (col < tokens ? col : tokens - 1) * stride + g * 16;
+    const uint8_t* const mine = lds + g * 16;        // (the one token, in every column)
     for (int chunk = 0; chunk < chunks; ++chunk) {
         i32x4_t now[U][NW], b[U][TT];
         int next[SHIFT ? U : 1][TT];
@@ -204,19 +199,8 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Few8Args a) 
 template <int XDT, bool PAIR, int NX, int TT, int RT, int WAVES>
 static int few8_as(const Few8Args& a, hipStream_t s) {
     constexpr int NW = RT * (PAIR ? 2 : 1);
-    const size_t partial = (size_t)WAVES * NW * TT * 1024, codes = NX > 0 ? (size_t)a.tokens * (a.kp + 16) : 0;
-    const size_t lds = partial > codes ? partial : codes;
-    const void* fn = (const void*)&int8_few_kernel<XDT, PAIR, NX, TT, RT, WAVES>;
-    if (lds > 64 * 1024) {
-        static bool raised[64];
-        int dev = 0;
-        (void)hipGetDevice(&dev);
-        if (dev < 0 || dev >= 64 || !raised[dev]) {
-            if (hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, 150 * 1024) != hipSuccess)
-                return fail(QMOE_ELAUNCH, "int8 product: the device refuses %zu bytes of LDS", lds);
-            if (dev >= 0 && dev < 64) raised[dev] = true;
-        }
-    }
+    const size_t partial = (size_t)WAVES * NW * TT * 1024, codes = NX > 0 ? (size_t)a.kp : 0;
+    const size_t lds = partial > codes ? partial : codes;            // (at most 32 KB)
     hipLaunchKernelGGL((int8_few_kernel<XDT, PAIR, NX, TT, RT, WAVES>), dim3((a.n + 16 * RT - 1) / (16 * RT), NX > 0 ? 1 : (a.tokens + 16 * TT - 1) / (16 * TT)), dim3(64 * WAVES), lds, s, a);
     return check_launch("int8 product of a few tokens");
 }

@@ -62,12 +62,13 @@ def int8_quantize(x):
     if x.dtype not in _TORCH_DTYPE_ID:
         raise TypeError("Rows to quantise must be FP16, BF16, or FP32")
     k = x.shape[-1]
-    if max(k, x.numel() // k) > _MOST:
+    rows = x.numel() // k
+    if k > _MOST or rows > _MOST:
         raise NotImplementedError(f"Rows to quantise: at most {_MOST} rows and columns")
     codes = torch.empty_like(x, dtype=torch.int8)
-    scales = x.new_empty(x.shape[:-1], dtype=torch.float32)
-    if x.numel():
-        rc = _call(x.device, _lib.load().qmoe_int8_quantize, x.data_ptr(), _TORCH_DTYPE_ID[x.dtype], x.numel() // k, k,
+    scales = x.new_empty(rows, dtype=torch.float32) if x.ndim == 2 else x.new_empty(x.shape[:-1], dtype=torch.float32)
+    if rows:
+        rc = _call(x.device, _lib.load().qmoe_int8_quantize, x.data_ptr(), _TORCH_DTYPE_ID[x.dtype], rows, k,
                    codes.data_ptr(), scales.data_ptr())
         if rc:
             _lib.check(rc, "Int8 quantisation")
@@ -144,7 +145,7 @@ def _codes_of(tiles, shape):
 
 
 def _activations(x, x_scales, k, device, out_dtype, what):
-    """(x's type id, scale address, output type) of a product's activations, checked."""
+    """(rows, x's type id, scale address, output type) of a product's activations, checked."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise TypeError(f"{what} must be a CUDA torch.Tensor")
     if x.ndim not in (2, 3):
@@ -155,7 +156,8 @@ def _activations(x, x_scales, k, device, out_dtype, what):
         raise ValueError("GPU input must be a contiguous tensor")
     if x.device != device:
         raise ValueError("all operands must be on the same device")
-    if x.numel() // k > _MOST:
+    m = x.numel() // k
+    if m > _MOST:
         raise NotImplementedError(f"{what}: at most {_MOST} rows")
     if out_dtype is not None and out_dtype not in _TORCH_DTYPE_ID:
         raise TypeError("out_dtype must be FP16, BF16, or FP32")
@@ -164,12 +166,12 @@ def _activations(x, x_scales, k, device, out_dtype, what):
             raise TypeError("int8 input needs x_scales, a torch.float32 tensor on its device")
         if x_scales.shape != x.shape[:-1] or not x_scales.is_contiguous():
             raise ValueError("x_scales must be contiguous with one scale for each row of x")
-        return _INT8, x_scales.data_ptr(), torch.float32 if out_dtype is None else out_dtype
+        return m, _INT8, x_scales.data_ptr(), torch.float32 if out_dtype is None else out_dtype
     if x.dtype not in _TORCH_DTYPE_ID:
         raise TypeError("GPU input must be FP16, BF16, FP32 or int8 codes")
     if x_scales is not None:
         raise ValueError("x_scales belong to int8 input")
-    return _TORCH_DTYPE_ID[x.dtype], None, x.dtype if out_dtype is None else out_dtype
+    return m, _TORCH_DTYPE_ID[x.dtype], None, x.dtype if out_dtype is None else out_dtype
 
 
 def int8_linear(x, weight, *, x_scales=None, out_dtype=None):
@@ -182,9 +184,8 @@ def int8_linear(x, weight, *, x_scales=None, out_dtype=None):
     if not isinstance(weight, Int8Weight):
         raise TypeError("Expected Int8Weight")
     n, k = weight.shape
-    xdt, sp, odt = _activations(x, x_scales, k, weight.device, out_dtype, "Int8 linear input")
-    m = x.numel() // k
-    out = x.new_empty((*x.shape[:-1], n), dtype=odt)
+    m, xdt, sp, odt = _activations(x, x_scales, k, weight.device, out_dtype, "Int8 linear input")
+    out = x.new_empty(m, n, dtype=odt) if x.ndim == 2 else x.new_empty((*x.shape[:-1], n), dtype=odt)
     if m:
         work, at, nbytes = _workspace(x, n, k, m, xdt)
         rc = _call(x.device, _lib.load().qmoe_int8_linear, weight.tiles.data_ptr(), weight.scales.data_ptr(), n, k, x.data_ptr(), xdt, sp,
@@ -203,9 +204,8 @@ def int8_swiglu(x, gate, up, *, x_scales=None, out_dtype=None):
     if gate.device != up.device:
         raise ValueError("all operands must be on the same device")
     f, k = gate.shape
-    xdt, sp, odt = _activations(x, x_scales, k, gate.device, out_dtype, "Int8 SwiGLU input")
-    m = x.numel() // k
-    out = x.new_empty((*x.shape[:-1], f), dtype=odt)
+    m, xdt, sp, odt = _activations(x, x_scales, k, gate.device, out_dtype, "Int8 SwiGLU input")
+    out = x.new_empty(m, f, dtype=odt) if x.ndim == 2 else x.new_empty((*x.shape[:-1], f), dtype=odt)
     if m:
         work, at, nbytes = _workspace(x, f, k, m, xdt)
         rc = _call(x.device, _lib.load().qmoe_int8_swiglu, gate.tiles.data_ptr(), gate.scales.data_ptr(), up.tiles.data_ptr(),

@@ -154,7 +154,8 @@ def test_linear_is_the_exact_sum_rounded_once(cuda, t, n, k, dtype):
 
 
 # sizes behind each of the tiles for many tokens, whole and with rests on every side; K from one column to many chunks
-TILED = [(950, 3590, 1), (960, 3584, 200), (1800, 4096, 64), (1790, 4090, 321), (4096, 4096, 72), (4001, 4085, 130), (700, 704, 1100), (690, 1000, 513)]
+TILED = [(950, 3590, 1), (960, 3584, 200), (1800, 4096, 64), (1790, 4090, 321), (4096, 4096, 72), (4001, 4085, 130), (700, 704, 1100), (690, 1000, 513),
+         (500, 3600, 330), (130, 1000, 2900), (140, 1001, 1700), (150, 990, 1300), (1000, 2000, 1500)]
 
 
 @pytest.mark.parametrize("t,n,k", TILED)
