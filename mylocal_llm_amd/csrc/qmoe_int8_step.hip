@@ -438,8 +438,7 @@ template <bool CODES> __global__ __launch_bounds__(BACK8_THREADS) void int8_back
     float* const scales = (float*)(sums + (size_t)(pairs + srows) * 16);
     float* const srow = scales + (size_t)(pairs + 1) * 16;
 
-    const int s_lo = a.fs_steps * wave / BACK8_WAVES, s_hi = a.fs_steps * (wave + 1) / BACK8_WAVES;
-    const uint8_t* const sp = a.fs ? a.s_down + (int64_t)tile * a.fsp * 16 + lane * 16 : nullptr;
+    const int n_active = __builtin_amdgcn_readfirstlane(ldg<int>(a.in.n_active));
     i32x4_t ring[BACK8_RING];
     // Codes: a wave a row, 512 values a turn.  A row's scale comes from the largest of each 16 channels, which the front kernel
     // left; four turns are requested at a time.  (Rows of pairs that do not count hold anything and are read by no result.)
@@ -467,7 +466,7 @@ template <bool CODES> __global__ __launch_bounds__(BACK8_THREADS) void int8_back
     };
     // with CODES: pieces of 16 bytes, first the pairs' rows, then the shared expert's
     const int h_pieces = pairs * a.f_steps * 4, pieces = h_pieces + srows * a.fs_steps * 4;
-    constexpr int NC = 4;
+    constexpr int NC = 8;
     i32x4_t piece[NC];
     auto fetch = [&](int p0) {
 #pragma unroll
@@ -481,7 +480,6 @@ template <bool CODES> __global__ __launch_bounds__(BACK8_THREADS) void int8_back
 #pragma unroll
         for (int p = 0; p < NX; ++p) load(wave + p * BACK8_WAVES, v[p], part[p]);
     }
-    const int n_active = *(const QMOE_GLOBAL int*)a.in.n_active;
     for (int i = tid; i < pairs; i += BACK8_THREADS) {
         pair_id[i] = ldg<int>(a.in.kept + i);
         pair_weight[i] = ldg<float>(a.in.weight + i);
@@ -489,10 +487,28 @@ template <bool CODES> __global__ __launch_bounds__(BACK8_THREADS) void int8_back
         active[i] = (uint16_t)ldg<int>(a.in.active + i);
     }
     for (int i = tid; i < pairs * 4; i += BACK8_THREADS) ((uint32_t*)slot_of)[i] = ldg<uint32_t>((const uint32_t*)a.in.slot + i);
-    // (requests come back in order: the weights' come last, so that nothing above waits for them)
-    if (s_lo < s_hi) {
+    // The list of steps: the shared expert's (item -1), then every chosen expert's.  The first requests leave before the codes are
+    // made; they come back in order, so that nothing above waits for them.
+    const int total = a.fs_steps + n_active * a.f_steps, lo = (int)((int64_t)total * wave / BACK8_WAVES), hi = (int)((int64_t)total * (wave + 1) / BACK8_WAVES);
+    const int64_t expert_bytes = (int64_t)((a.d + 15) / 16) * a.fp * 16;
+    const int lo_ai = lo < a.fs_steps ? -1 : (lo - a.fs_steps) / a.f_steps, lo_k = lo_ai < 0 ? lo : lo - a.fs_steps - lo_ai * a.f_steps;
+    int f_ai = lo_ai, f_k = lo_k, f_end = lo_ai < 0 ? a.fs_steps : a.f_steps, left = hi - lo;
+    const uint8_t* pw = nullptr;
+    auto point = [&](int e) {
+        pw = (f_ai < 0 ? a.s_down + (int64_t)tile * a.fsp * 16 : a.down + e * expert_bytes + (int64_t)tile * a.fp * 16) + (int64_t)f_k * 1024;
+    };
+    auto request = [&](int u, auto&& expert_at) {
+        ring[u] = ldg_i32x4(pw + lane * 16);
+        if (--left > 0) {                      // (past the end the last step is requested again)
+            pw += 1024;
+            if (++f_k == f_end) { f_k = 0; ++f_ai; f_end = a.f_steps; point(expert_at(f_ai)); }
+        }
+    };
+    if (lo < hi) {
+        auto listed = [&](int ai) { return __builtin_amdgcn_readfirstlane(ldg<int>(a.in.active + ai)); };
+        point(f_ai < 0 ? 0 : listed(f_ai));
 #pragma unroll
-        for (int u = 0; u < BACK8_RING; ++u) ring[u] = ldg_i32x4(sp + (int64_t)(s_lo + u < s_hi ? s_lo + u : s_hi - 1) * 1024);
+        for (int u = 0; u < BACK8_RING; ++u) request(u, listed);
     }
     for (int i = tid; i < rows * 16; i += BACK8_THREADS) sums[i] = 0;
     if (CODES) {
@@ -549,45 +565,17 @@ template <bool CODES> __global__ __launch_bounds__(BACK8_THREADS) void int8_back
 #pragma unroll
         for (int i = 0; i < 4; ++i) atomicAdd(s + i, acc[i]);
     };
-    // ---- shared expert ----
-    if (s_lo < s_hi) {
-        const uint8_t* const b0 = sq + (size_t)(col < tokens ? col : tokens - 1) * sst + g * 16;
-        i32x4_t acc = {0, 0, 0, 0};
-        int s = s_lo;
-        for (; s + BACK8_RING <= s_hi; s += BACK8_RING)
-#pragma unroll
-            for (int u = 0; u < BACK8_RING; ++u) {
-                acc = mfma_i8(ring[u], *(const i32x4_t*)(b0 + (s + u) * 64), acc);
-                ring[u] = ldg_i32x4(sp + (int64_t)(s + u + BACK8_RING < s_hi ? s + u + BACK8_RING : s_hi - 1) * 1024);
-            }
-#pragma unroll
-        for (int u = 0; u + 1 < BACK8_RING; ++u)
-            if (s + u < s_hi) acc = mfma_i8(ring[u], *(const i32x4_t*)(b0 + (s + u) * 64), acc);
-        if (col < tokens) add(pairs + col, acc);
-    }
-    // ---- the chosen experts ----
-    const int total = n_active * a.f_steps, lo = (int)((int64_t)total * wave / BACK8_WAVES), hi = (int)((int64_t)total * (wave + 1) / BACK8_WAVES);
+    // ---- stream ----
     if (lo < hi) {
-        const int64_t expert_bytes = (int64_t)((a.d + 15) / 16) * a.fp * 16;
-        int f_ai = lo / a.f_steps, f_k = lo - f_ai * a.f_steps, left = hi - lo;
-        const uint8_t* pw;
-        auto point = [&]() {
-            const int e = __builtin_amdgcn_readfirstlane((int)active[f_ai]);
-            pw = a.down + e * expert_bytes + (int64_t)tile * a.fp * 16 + (int64_t)f_k * 1024;
-        };
-        point();
-        auto request = [&](int u) {
-            ring[u] = ldg_i32x4(pw + lane * 16);
-            if (--left > 0) {
-                pw += 1024;
-                if (++f_k == a.f_steps) { f_k = 0; ++f_ai; point(); }
-            }
-        };
-#pragma unroll
-        for (int u = 0; u < BACK8_RING; ++u) request(u);
-        int c_ai = lo / a.f_steps, c_k = lo - c_ai * a.f_steps, p = -1;
+        auto listed = [&](int ai) { return __builtin_amdgcn_readfirstlane((int)active[ai]); };
+        int c_ai = lo_ai, c_k = lo_k, c_end = lo_ai < 0 ? a.fs_steps : a.f_steps, p = -1;
         const uint8_t* b0 = hq;
         auto enter = [&]() {       // this lane's token's row of codes, a valid one where the token did not choose the expert
+            if (c_ai < 0) {
+                p = col < tokens ? pairs + col : -1;
+                b0 = sq + (size_t)(col < tokens ? col : 0) * sst + g * 16;
+                return;
+            }
             const int s = col < tokens ? slot_of[c_ai * STEP8_TOKENS + col] : 255;
             p = s < 255 ? col * k + s : -1;
             b0 = hq + (size_t)(p < 0 ? 0 : p) * hst + g * 16;
@@ -596,17 +584,18 @@ template <bool CODES> __global__ __launch_bounds__(BACK8_THREADS) void int8_back
         i32x4_t acc = {0, 0, 0, 0};
         auto multiply = [&](int u) {
             acc = mfma_i8(ring[u], *(const i32x4_t*)(b0 + c_k * 64), acc);
-            if (++c_k == a.f_steps) {
+            if (++c_k == c_end) {
                 if (p >= 0) add(p, acc);
                 acc = i32x4_t{0, 0, 0, 0};
                 c_k = 0;
+                c_end = a.f_steps;
                 if (++c_ai < n_active) enter();
             }
         };
         int s = lo;
         for (; s + BACK8_RING <= hi; s += BACK8_RING)
 #pragma unroll
-            for (int u = 0; u < BACK8_RING; ++u) { multiply(u); request(u); }
+            for (int u = 0; u < BACK8_RING; ++u) { multiply(u); request(u, listed); }
 #pragma unroll
         for (int u = 0; u + 1 < BACK8_RING; ++u)
             if (s + u < hi) multiply(u);
