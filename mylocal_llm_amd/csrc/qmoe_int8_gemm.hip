@@ -112,32 +112,34 @@ __global__ __launch_bounds__(64 * WN * WT) __attribute__((amdgpu_waves_per_eu(2)
     const uint8_t* const mine0 = lds + wt * (TT * 16 * KC) + (g * 16 + (col ^ swap(g))) * 16;
     const uint8_t* const mine1 = lds + wt * (TT * 16 * KC) + (g * 16 + (col ^ swap(g | 4))) * 16;
     constexpr int TH = TT / 2;        // tokens' tiles of half a step
-    i32x4_t b[2][TH];
+    constexpr int D = TT <= 4 ? 4 : 2, HALVES = 2 * KK;
+    static_assert(HALVES % D == 0, "a chunk turns the operands' ring whole");
+    i32x4_t b[D][TH];
     auto read_b = [&](int buffer, int half, i32x4_t (&to)[TH]) {
         const int kk = half / 2;
 #pragma unroll
         for (int t = 0; t < TH; ++t)
             to[t] = *(const i32x4_t*)((kk & 1 ? mine1 : mine0) + (buffer * (ROWS * KC) + ((half % 2 * TH + t) * KK + kk) * 1024));
     };
-    // A chunk in halves of a step: while one half is multiplied the next half's operands are read, and the last half of a
-    // chunk is multiplied behind the meeting that opens the next one.  A step's weights are requested again into the
-    // registers they leave, R steps ahead; activations are requested XR + 1 chunks ahead of their use.
+    // A chunk in halves of a step: while one half is multiplied the operands of the next D - 1 are on their way from LDS, and
+    // the last D - 1 halves of a chunk are multiplied behind the meeting that opens the next one.  (Small tiles multiply a half
+    // in less time than LDS answers in: D = 4 instead of 2 takes 512 x 2048 x 2048 from 7.9 to 7.1 us, 64 x 4096 x 4096 from 8.8 to
+    // 8.5.)  A step's weights are requested again into the registers they leave, R steps ahead; activations are requested XR + 1
+    // chunks ahead of their use.
     auto turn = [&](int c, int h) {
         keep_x((h + 1) & 1, xr[(h + 1) % XR]);
         request_x(c + 1 + XR, xr[(h + 1) % XR]);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < 2 * KK; ++j) {
-            if (j + 1 < 2 * KK) read_b(h & 1, j + 1, b[(j + 1) & 1]);
-            else {
-                meet_lds();
-                read_b((h + 1) & 1, 0, b[0]);
-            }
+        for (int j = 0; j < HALVES; ++j) {
+            const int ahead = j + D - 1;
+            if (ahead == HALVES) meet_lds();
+            read_b((ahead < HALVES ? h : h + 1) & 1, ahead % HALVES, b[ahead % D]);
             i32x4_t(&w)[NW] = wr[(h * KK + j / 2) % R];
 #pragma unroll
             for (int t = 0; t < TH; ++t)
 #pragma unroll
-                for (int i = 0; i < NW; ++i) acc[i][j % 2 * TH + t] = mfma_i8(w[i], b[j & 1][t], acc[i][j % 2 * TH + t]);
+                for (int i = 0; i < NW; ++i) acc[i][j % 2 * TH + t] = mfma_i8(w[i], b[j % D][t], acc[i][j % 2 * TH + t]);
             if (j & 1) request_w(c * KK + j / 2 + R, w);
             __builtin_amdgcn_sched_barrier(0);     // (the scheduler would gather the requests behind the products)
         }
@@ -150,7 +152,8 @@ __global__ __launch_bounds__(64 * WN * WT) __attribute__((amdgpu_waves_per_eu(2)
 #pragma unroll
     for (int r = 0; r < R; ++r) request_w(r, wr[r]);
     meet_lds();
-    read_b(0, 0, b[0]);
+#pragma unroll
+    for (int j = 0; j + 1 < D; ++j) read_b(0, j, b[j]);
     // whole rounds without a condition inside: one would make the compiler move registers that are still on their way, and
     // wait for them
     int c0 = 0;
@@ -275,7 +278,7 @@ int int8_plan_launch(const Int8Product& a, bool pair, int rows, int max_chunks, 
 // The largest tile that still gives nearly every CU a workgroup (us from codes; 256 x 256 of eight waves / 256 channels x
 // 128 tokens of four, two workgroups a CU / 256 x 64 / 128 x 64 / 64 x 64 / 64 x 32 / 32 x 32): 4096 tokens x 4096 x 14336
 // 184 / 184 / 220 / - / 351, 4096 x 14336 x 4096 225 / 213 / 268 / - / 380, 512 x 14336 x 4096 49 / 33 / 36 / - / 48,
-// 1024 x 4096 x 4096 47 / 30 / 22 / 25 / 29, 128 x 14336 x 4096 - / - / 29 / 20 / 22 / 28, 512 x 2048 x 2048 - / - / 12 / 9.2 / 7.5 /
+// 1024 x 4096 x 4096 47 / 30 / 22 / 25 / 29, 128 x 14336 x 4096 - / - / 29 / 20 / 22 / 28, 512 x 2048 x 2048 - / - / 12 / 9.2 / 7.1 /
 // 7.7, 128 x 4096 x 4096 - / - / 18 / 13 / 12.4 / 10.0 / 12.2, 64 x 4096 x 14336 - / - / - / - / 35 / 27 / 20.
 // One workgroup a CU loses what the last round leaves empty, and nothing hides its start and its end: the largest tile is
 // taken where the rounds come out nearly even.

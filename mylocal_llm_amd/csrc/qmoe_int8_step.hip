@@ -14,9 +14,9 @@
 // another inside the stream.  Requests run R steps ahead through a ring of registers.
 //
 // Measured at 512 experts, ten a token, 2048 columns, width 512, shared expert of 2048, weights from memory:
-//   1 token    front 13.6 us, back 9.6 us for 44 MB: two launches, each a chain of latencies (launch 2, logits and rows 2,
+//   1 token    front 13.6 us, back 9.4 us for 44 MB: two launches, each a chain of latencies (launch 2, logits and rows 2,
 //              selection 1, first weights 2 us) around 4 - 5 us of streaming
-//   16 tokens  routing 6.0, front 61.6 (300 MB, 4.9 TB/s), codes 4.7, back 35.5 us (150 MB, 4.2 TB/s)
+//   16 tokens  routing 6.0, front 61.6 (300 MB, 4.9 TB/s), codes 4.7, back 34.6 us (150 MB, 4.3 TB/s)
 #include "qmoe_int8_route.hpp"
 
 namespace qmoe {
