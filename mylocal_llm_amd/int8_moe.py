@@ -48,11 +48,14 @@ class Int8ExpertBank:
         self.gate_scales, self.up_scales, self.down_scales = scales
         self.n_experts, self.d_model, self.d_ff = e, d, f
         self.device = tiles[0].device
-        # the step's argument struct with what never changes filled in; a call copies it
-        a = self._args = _lib.Int8MoeArgs()
-        a.gate, a.up, a.down = (m.data_ptr() for m in tiles)
-        a.gate_scales, a.up_scales, a.down_scales = (m.data_ptr() for m in scales)
-        a.n_experts, a.d_model, a.d_ff = e, d, f
+
+    def fill(self, args):
+        """The bank's part of a step's argument struct.  Addresses are read from the tensors at every call: one kept from an
+        earlier call would be stale, or free, once a tensor is replaced."""
+        args.gate, args.up, args.down = self.gate_tiles.data_ptr(), self.up_tiles.data_ptr(), self.down_tiles.data_ptr()
+        args.gate_scales, args.up_scales, args.down_scales = (
+            self.gate_scales.data_ptr(), self.up_scales.data_ptr(), self.down_scales.data_ptr())
+        args.n_experts, args.d_model, args.d_ff = self.n_experts, self.d_model, self.d_ff
 
     @classmethod
     def from_packed(cls, bank):
@@ -138,7 +141,8 @@ def int8_moe_step(hidden, bank, top_k, *, logits=None, weights=None, ids=None, s
     t, k = hidden.shape[0], int(top_k)
     if not 1 <= k <= min(32, e) or e > 4096:
         raise NotImplementedError("the step covers at most 4096 experts and 1 <= top_k <= min(32, experts)")
-    args = _lib.Int8MoeArgs.from_buffer_copy(bank._args)
+    args = _lib.Int8MoeArgs()
+    bank.fill(args)
     lg = iw = ii = rs = None
     if logits is not None:
         lg = _given(logits, torch.float32, (t, e), device, "router logits")
