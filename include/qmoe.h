@@ -295,8 +295,8 @@ int qmoe_read_probe(const void* buffer, size_t bytes, uint32_t match, uint32_t* 
  * counterpart in the reference, whose packed products keep activations in floating point.
  *     q[t, k] = rint(x[t, k] / s[t]),  s[t] = fl32(max_k |x[t, k]| / 127)   halves to even, |q| <= 127
  *     y[t, n] = (sum_k q[t, k] w[n, k]) * s[t] * c[n]                       int32 sum, exact
- * The scales are applied in 64 bits and the result rounded to fp32, then to y's type (16-bit results of
- * many tokens: scaled in fp32 where s c is in its normal range).
+ * The scales are applied in 64 bits and the result rounded to fp32, then to y's type: its bits depend on
+ * its own row and channel only, not on the number of tokens, the other rows or y's address.
  * s[t] == 0 makes all codes 0; a row with a NaN or an infinity gets s[t] = NaN and codes of 0, so its
  * products are NaN.  Weights are any int8 codes with fp32 scales, laid out once as tiles of 16
  * channels x 64 columns (qmoe_int8_tiles), zero-padded.  K <= 131071, where the int32 sum cannot

@@ -122,10 +122,18 @@ template <int DT> __device__ __forceinline__ void int8_load8(const void* x, size
 // acc * s * c with one rounding that counts: the sum has up to 31 bits, the scales 24 each.
 __device__ __forceinline__ double int8_value(int acc, float s, float c) { return (double)acc * ((double)s * (double)c); }
 
+// v rounded to fp32, and to nothing else: a conversion of the result to 16 bits must not be joined with this one (the compiler
+// contracts the two to one rounding, in software for fp16, on one path and not on another).
+__device__ __forceinline__ float to_fp32(double v) {
+    float f = (float)v;
+    asm("" : "+v"(f));
+    return f;
+}
+
 // silu(g) * u in 64 bits.  The activation that an expert hands to its down projection is rounded to
 // fp32 from this and then cut into codes: every kernel forms it the same way, so that a value next to
 // the border of two codes gets the same code however many tokens share the step.
-__device__ __forceinline__ float int8_hidden(double g, double u) { return (float)(g / (1.0 + exp(-g)) * u); }
+__device__ __forceinline__ float int8_hidden(double g, double u) { return to_fp32(g / (1.0 + exp(-g)) * u); }
 
 // LDS operations of this workgroup's waves before and after; requests for memory stay in flight.
 __device__ __forceinline__ void meet_lds() {

@@ -191,7 +191,7 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Few8Args a) 
             if (PAIR) s1 += part[(size_t)(w * NW + r * NP + 1) * TT * 256 + at];
         }
         const double v = int8_value(s0, srow[t], a.c[n]);
-        const float out = PAIR ? int8_hidden(v, int8_value(s1, srow[t], a.c2[n])) : (float)v;
+        const float out = PAIR ? int8_hidden(v, int8_value(s1, srow[t], a.c2[n])) : to_fp32(v);
         store_out(a.y, a.ydt, (size_t)(first + t) * a.n + n, out);
     }
 }

@@ -2,8 +2,9 @@
 
 Both sides are int8: weights with a scale for each output channel, activations with a scale for each
 token, quantised on the way (``int8_quantize``) or given as codes.  The sum of code products is exact
-in int32, so a result is ``(sum q w) * s * c`` to one rounding of the output type, whatever the number of
-tokens (16-bit results of many tokens are scaled in fp32, three roundings of 2^-24, before it).  The reference keeps activations in floating point (mini_llm/ops/quantized_linear.py:272-400);
+in int32 and scaled in 64 bits, so a result is ``(sum q w) * s * c`` rounded to fp32 and then to the output
+type; its bits depend on its own row and channel only, not on the number of tokens, the other rows or where it
+lies.  The reference keeps activations in floating point (mini_llm/ops/quantized_linear.py:272-400);
 these operators stand beside ``quantized_linear`` / ``quantized_swiglu``, which take an ``Int8Weight``
 wherever they take a packed GGUF weight.
 """

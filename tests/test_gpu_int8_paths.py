@@ -1,0 +1,94 @@
+"""The 8-bit integer products take several kernels, by their sizes; a value's bits may depend on none of that.
+
+Sizes are chosen so that the tiles of many tokens are what runs, and ``tiled`` asserts it: codes need a workspace only there.
+(A pair is taken by the few-token kernel up to 256 blocks of 16 channels x 32 tokens.)
+"""
+import pytest
+import torch
+
+from mylocal_llm_amd import _lib
+from mylocal_llm_amd.int8_linear import Int8Weight, int8_linear, int8_quantize, int8_swiglu
+from mylocal_llm_amd.quantized_linear import _TORCH_DTYPE_ID
+from gpu_util import announce
+from test_gpu_int8 import DTYPES, matrix, rows
+
+pytestmark = pytest.mark.gpu
+INT8 = 3
+
+
+def tiled(t, n, k):
+    """Both a product and a pair of these sizes run on the tiles of many tokens."""
+    assert _lib.load().qmoe_int8_workspace_bytes(n, k, t, INT8) > 0 and (n + 15) // 16 * ((t + 31) // 32) > 256
+
+
+def pair_of(n, k, seed):
+    g, u = matrix(n, k, seed), matrix(n, k, seed + 1)
+    g[1].mul_(20.0 / k ** 0.5)
+    return g, u
+
+
+def both(gate, up, dtype):
+    return [("linear", lambda x, s: int8_linear(x, gate, x_scales=s, out_dtype=dtype)),
+            ("swiglu", lambda x, s: int8_swiglu(x, gate, up, x_scales=s, out_dtype=dtype))]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,n,k", [(512, 2048, 256), (300, 2000, 200), (4096, 4096, 64)])
+def test_a_row_does_not_move_its_neighbours_bits(cuda, t, n, k, dtype):
+    """Rows whose scale is NaN, infinite, tiny, huge or 0 between ordinary ones: the others keep every bit."""
+    announce("int8 neighbours", t, n, k, dtype)
+    tiled(t, n, k)
+    g, u = pair_of(n, k, t + n)
+    codes, scales = int8_quantize(rows(t, k, t))
+    for name, call in both(Int8Weight(*g), Int8Weight(*u), dtype):
+        clean = call(codes, scales)
+        odd = torch.arange(7, t, 37, device=cuda)
+        keep = torch.ones(t, dtype=torch.bool, device=cuda)
+        keep[odd] = False
+        for bad in (float("nan"), float("inf"), 1e-30, 1e30, 0.0):
+            s = scales.clone()
+            s[odd] = bad
+            got = call(codes, s)
+            assert torch.equal(got[keep], clean[keep]), (name, bad, int((got[keep] != clean[keep]).sum()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,n,k", [(512, 2048, 256), (300, 2000, 200), (4096, 4096, 64), (700, 3600, 1000), (100, 1601, 96)])
+def test_a_token_alone_and_in_a_prompt_gets_the_same_bits(cuda, t, n, k, dtype):
+    announce("int8 alone and in a prompt", t, n, k, dtype)
+    tiled(t, n, k)
+    g, u = pair_of(n, k, t + k)
+    codes, scales = int8_quantize(rows(t, k, t))
+    for name, call in both(Int8Weight(*g), Int8Weight(*u), dtype)[:1]:
+        whole = call(codes, scales)
+        for lo, hi in ((0, 1), (1, 17), (t - 16, t), (t // 2, t // 2 + 5)):
+            part = call(codes[lo:hi].contiguous(), scales[lo:hi].contiguous())
+            assert torch.equal(part, whole[lo:hi]), (name, lo, hi, int((part != whole[lo:hi]).sum()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,n,k", [(512, 2048, 256), (300, 2000, 200), (4096, 4096, 64)])
+def test_a_values_bits_do_not_depend_on_where_it_lies(cuda, t, n, k, dtype):
+    """The last blocks of a narrower matrix, rows that start anywhere, an output at an odd address."""
+    announce("int8 places", t, n, k, dtype)
+    g, u = pair_of(n, k, t + 3)
+    codes, scales = int8_quantize(rows(t, k, t))
+    lib, stream = _lib.load(), torch.cuda.current_stream().cuda_stream
+    work = torch.empty(lib.qmoe_int8_workspace_bytes(n, k, t, INT8), dtype=torch.uint8, device=cuda)
+    gate, up = Int8Weight(*g), Int8Weight(*u)
+    whole = [call(codes, scales) for _, call in both(gate, up, dtype)]
+    for m in (n - 1, n - 14, n - 100, n // 2 + 602):
+        tiled(t, m, k)
+        parts = [Int8Weight(w[0][:m].contiguous(), w[1][:m].contiguous()) for w in (g, u)]
+        for (name, call), want in zip(both(*parts, dtype)[:1], whole):
+            got = call(codes, scales)
+            assert torch.equal(got, want[:, :m]), (name, m, int((got != want[:, :m]).sum()))
+    base = torch.full((t * n + 2,), 3.0, dtype=dtype, device=cuda)
+    odt = _TORCH_DTYPE_ID[dtype]
+    for pair, want in enumerate(whole[:1]):
+        head = [gate.tiles.data_ptr(), gate.scales.data_ptr()] + ([up.tiles.data_ptr(), up.scales.data_ptr()] if pair else [])
+        entry = lib.qmoe_int8_swiglu if pair else lib.qmoe_int8_linear
+        base.fill_(3.0)
+        assert entry(*head, n, k, codes.data_ptr(), INT8, scales.data_ptr(), t, base[1:].data_ptr(), odt, work.data_ptr(), work.numel(), stream) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(base[1:-1].reshape(t, n), want) and base[0] == 3 and base[-1] == 3
