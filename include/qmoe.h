@@ -324,7 +324,7 @@ int qmoe_int8_linear(const void* tiles, const float* channel_scales, int n, int 
                      const float* x_scales, int tokens, void* y, int y_dtype, void* workspace,
                      size_t workspace_bytes, void* stream);
 
-/* h[tokens, f] = silu(x @ G^T) * (x @ U^T) on the same terms; gate and up share [f, k]. */
+/* h[tokens, f] = silu(x @ G^T) * (x @ U^T) on the same terms, silu in 64 bits; gate and up share [f, k]. */
 int qmoe_int8_swiglu(const void* gate, const float* gate_scales, const void* up, const float* up_scales, int f, int k,
                      const void* x, int x_dtype, const float* x_scales, int tokens, void* h, int h_dtype,
                      void* workspace, size_t workspace_bytes, void* stream);

@@ -130,10 +130,33 @@ __device__ __forceinline__ float to_fp32(double v) {
     return f;
 }
 
-// silu(g) * u in 64 bits.  The activation that an expert hands to its down projection is rounded to
-// fp32 from this and then cut into codes: every kernel forms it the same way, so that a value next to
-// the border of two codes gets the same code however many tokens share the step.
-__device__ __forceinline__ float int8_hidden(double g, double u) { return to_fp32(g / (1.0 + exp(-g)) * u); }
+// silu(g) * u = g u / (1 + 2^y), y = -g log2 e, in 64 bits and rounded to fp32: the one formula of every kernel.  The activation
+// that an expert hands to its down projection is cut into codes: a value next to the border of two codes gets the same code
+// however many tokens share the step, and a SwiGLU's value the same bits.
+//   2^y = 2^n 2^r, n = rint(y), |r| <= 1/2;  2^r = 1 + r P(r), P of degree 9 through (2^r - 1) / r at ten Chebyshev nodes: 2^-50.6
+//   1 / (1 + 2^y): the instruction's 2^-24, one Newton step
+// y's own rounding counts |y| 2^-53 ln 2, so silu is off by 2^-46 at most for |g| up to 110, beyond which |silu| is below 2^-150.
+// y below -1000 adds nothing to 1, and 2^n is cut at 2^1000, where silu(g) u is far below fp32 (|g u| < 2^574); g = -infinity and
+// NaN give NaN.  Half the instructions of exp and a division in 64 bits: SwiGLU 4096 x 14336 x 64 bf16 from codes 94 us instead of 128
+// (silu in fp32: 91), 4096 x 4096 x 512 39 instead of 51.
+__device__ __forceinline__ float int8_hidden(double g, double u) {
+    const double y = fmax(g * -0x1.71547652b82fep+0, -1000.0), n = __builtin_rint(y), r = y - n;
+    double p = 0x1.e5e9f548e5726p-28;
+    p = __builtin_fma(p, r, 0x1.b6571de2f2351p-24);
+    p = __builtin_fma(p, r, 0x1.62bfe46117445p-20);
+    p = __builtin_fma(p, r, 0x1.ffcb76789860fp-17);
+    p = __builtin_fma(p, r, 0x1.4309130378460p-13);
+    p = __builtin_fma(p, r, 0x1.5d87fe908f88ap-10);
+    p = __builtin_fma(p, r, 0x1.3b2ab6fba385fp-7);
+    p = __builtin_fma(p, r, 0x1.c6b08d7044119p-5);
+    p = __builtin_fma(p, r, 0x1.ebfbdff82c590p-3);
+    p = __builtin_fma(p, r, 0x1.62e42fefa39f7p-1);
+    p = __builtin_fma(p, r, 1.0);
+    const double d = 1.0 + ldexp(p, (int)fmin(n, 1000.0));
+    double i = __builtin_amdgcn_rcp(d);
+    i = __builtin_fma(__builtin_fma(-d, i, 1.0), i, i);
+    return to_fp32(g * i * u);
+}
 
 // LDS operations of this workgroup's waves before and after; requests for memory stay in flight.
 __device__ __forceinline__ void meet_lds() {

@@ -13,7 +13,7 @@
 namespace qmoe {
 
 // R: steps of 64 columns that the weights' requests run ahead; XR: chunks that the activations' requests run ahead.
-template <bool PAIR, bool HIDDEN, bool PLAN, int WN, int WT, int RT, int TT, int KC, int R, int XR>
+template <bool PAIR, bool PLAN, int WN, int WT, int RT, int TT, int KC, int R, int XR>
 __global__ __launch_bounds__(64 * WN * WT) __attribute__((amdgpu_waves_per_eu(2))) void int8_gemm_kernel(const Int8Product main_args, int n_blocks, int t_blocks,
                                                                  const Int8Product side_args, int side_n, int side_t) {
     constexpr int THREADS = 64 * WN * WT, NP = PAIR ? 2 : 1, NW = RT * NP;
@@ -171,7 +171,7 @@ __global__ __launch_bounds__(64 * WN * WT) __attribute__((amdgpu_waves_per_eu(2)
         const double y = (double)acc[i * NP][t][j] * ((double)s * c);
         if (!PAIR) return to_fp32(y);
         const double u = (double)acc[i * NP + 1][t][j] * ((double)s * c2);
-        return HIDDEN ? int8_hidden(y, u) : silu_mul(to_fp32(y), to_fp32(u));
+        return int8_hidden(y, u);
     };
     const int n0 = (bn * WN + wn) * RT * 16 + 4 * g;
     double c[RT][4], c2[RT][4];
@@ -232,13 +232,13 @@ __global__ __launch_bounds__(64 * WN * WT) __attribute__((amdgpu_waves_per_eu(2)
     }
 }
 
-template <bool PAIR, bool HIDDEN, bool PLAN, int WN, int WT, int RT, int TT, int KC, int R, int XR>
+template <bool PAIR, bool PLAN, int WN, int WT, int RT, int TT, int KC, int R, int XR>
 static int gemm8_as(const Int8Product& a, int chunks, hipStream_t s, const Int8Product* side = nullptr) {
     const int nb = (a.n + 16 * WN * RT - 1) / (16 * WN * RT), tb = PLAN ? (chunks + 31) / 32 * 32 : (a.tokens + 16 * WT * TT - 1) / (16 * WT * TT);
     const int sn = side ? (side->n + 16 * WN * RT - 1) / (16 * WN * RT) : 0, st = side ? (side->tokens + 16 * WT * TT - 1) / (16 * WT * TT) : 0;
     if (((int64_t)nb * tb + (int64_t)sn * st) * (64 * WN * WT) > 0xFFFFFFFFll)      // (a launch's threads are counted in 32 bits)
         return fail(QMOE_EUNSUPPORTED, "int8 product: %d x %d blocks exceed a launch; split the tokens", nb, tb);
-    hipLaunchKernelGGL((int8_gemm_kernel<PAIR, HIDDEN, PLAN, WN, WT, RT, TT, KC, R, XR>), dim3(nb * tb + sn * st), dim3(64 * WN * WT), 0, s, a, nb, PLAN ? chunks : tb,
+    hipLaunchKernelGGL((int8_gemm_kernel<PAIR, PLAN, WN, WT, RT, TT, KC, R, XR>), dim3(nb * tb + sn * st), dim3(64 * WN * WT), 0, s, a, nb, PLAN ? chunks : tb,
                        side ? *side : a, sn, st);
     return check_launch("int8 product");
 }
@@ -253,13 +253,13 @@ int int8_plan_rows(int64_t assignments, int n_experts) {
 // side: NULL, or a dense product of the same kind (pair with the hidden activation, or plain) that rides in front.
 int int8_plan_launch(const Int8Product& a, bool pair, int rows, int max_chunks, const Int8Product* side, hipStream_t s) {
     if (pair) {
-        if (rows == 32) return gemm8_as<true, true, true, 4, 1, 1, 2, 256, 8, 2>(a, max_chunks, s, side);
-        if (rows == 64) return gemm8_as<true, true, true, 4, 1, 1, 4, 256, 8, 1>(a, max_chunks, s, side);
-        return gemm8_as<true, true, true, 4, 1, 2, 8, 128, 4, 1>(a, max_chunks, s, side);
+        if (rows == 32) return gemm8_as<true, true, 4, 1, 1, 2, 256, 8, 2>(a, max_chunks, s, side);
+        if (rows == 64) return gemm8_as<true, true, 4, 1, 1, 4, 256, 8, 1>(a, max_chunks, s, side);
+        return gemm8_as<true, true, 4, 1, 2, 8, 128, 4, 1>(a, max_chunks, s, side);
     }
-    if (rows == 32) return gemm8_as<false, false, true, 4, 1, 2, 2, 256, 4, 2>(a, max_chunks, s, side);
-    if (rows == 64) return gemm8_as<false, false, true, 4, 1, 2, 4, 256, 8, 1>(a, max_chunks, s, side);
-    return gemm8_as<false, false, true, 4, 1, 4, 8, 128, 4, 1>(a, max_chunks, s, side);
+    if (rows == 32) return gemm8_as<false, true, 4, 1, 2, 2, 256, 4, 2>(a, max_chunks, s, side);
+    if (rows == 64) return gemm8_as<false, true, 4, 1, 2, 4, 256, 8, 1>(a, max_chunks, s, side);
+    return gemm8_as<false, true, 4, 1, 4, 8, 128, 4, 1>(a, max_chunks, s, side);
 }
 
 // The largest tile that still gives nearly every CU a workgroup (us from codes; 256 x 256 of eight waves / 256 channels x
@@ -279,17 +279,17 @@ int int8_gemm_launch(const Int8Product& a, bool pair, hipStream_t s) {
     const int wide = pair ? 128 : 256;
     const int64_t large = blocks(wide, 256), rounds = (large + CUS - 1) / CUS * CUS;
     if (large >= ENOUGH && large * 20 >= rounds * 19)
-        return pair ? gemm8_as<true, false, false, 4, 2, 2, 8, 128, 4, 1>(a, 0, s) : gemm8_as<false, false, false, 4, 2, 4, 8, 128, 4, 1>(a, 0, s);
+        return pair ? gemm8_as<true, false, 4, 2, 2, 8, 128, 4, 1>(a, 0, s) : gemm8_as<false, false, 4, 2, 4, 8, 128, 4, 1>(a, 0, s);
     if (blocks(wide, 128) >= ENOUGH)
-        return pair ? gemm8_as<true, false, false, 4, 1, 2, 8, 128, 4, 1>(a, 0, s) : gemm8_as<false, false, false, 4, 1, 4, 8, 128, 4, 1>(a, 0, s);
+        return pair ? gemm8_as<true, false, 4, 1, 2, 8, 128, 4, 1>(a, 0, s) : gemm8_as<false, false, 4, 1, 4, 8, 128, 4, 1>(a, 0, s);
     if (blocks(wide, 64) >= ENOUGH)
-        return pair ? gemm8_as<true, false, false, 4, 1, 2, 4, 128, 4, 1>(a, 0, s) : gemm8_as<false, false, false, 4, 1, 4, 4, 128, 4, 1>(a, 0, s);
-    if (!pair && blocks(128, 64) >= ENOUGH) return gemm8_as<false, false, false, 4, 1, 2, 4, 256, 8, 1>(a, 0, s);
+        return pair ? gemm8_as<true, false, 4, 1, 2, 4, 128, 4, 1>(a, 0, s) : gemm8_as<false, false, 4, 1, 4, 4, 128, 4, 1>(a, 0, s);
+    if (!pair && blocks(128, 64) >= ENOUGH) return gemm8_as<false, false, 4, 1, 2, 4, 256, 8, 1>(a, 0, s);
     if (blocks(64, 64) >= ENOUGH)
-        return pair ? gemm8_as<true, false, false, 4, 1, 1, 4, 256, 8, 2>(a, 0, s) : gemm8_as<false, false, false, 4, 1, 1, 4, 256, 8, 1>(a, 0, s);
+        return pair ? gemm8_as<true, false, 4, 1, 1, 4, 256, 8, 2>(a, 0, s) : gemm8_as<false, false, 4, 1, 1, 4, 256, 8, 1>(a, 0, s);
     if (blocks(64, 32) >= 192)
-        return pair ? gemm8_as<true, false, false, 4, 1, 1, 2, 256, 8, 2>(a, 0, s) : gemm8_as<false, false, false, 4, 1, 1, 2, 256, 8, 2>(a, 0, s);
-    return pair ? gemm8_as<true, false, false, 2, 1, 1, 2, 256, 16, 4>(a, 0, s) : gemm8_as<false, false, false, 2, 1, 1, 2, 256, 16, 4>(a, 0, s);
+        return pair ? gemm8_as<true, false, 4, 1, 1, 2, 256, 8, 2>(a, 0, s) : gemm8_as<false, false, 4, 1, 1, 2, 256, 8, 2>(a, 0, s);
+    return pair ? gemm8_as<true, false, 2, 1, 1, 2, 256, 16, 4>(a, 0, s) : gemm8_as<false, false, 2, 1, 1, 2, 256, 16, 4>(a, 0, s);
 }
 
 }  // namespace qmoe

@@ -197,7 +197,8 @@ def int8_linear(x, weight, *, x_scales=None, out_dtype=None):
 
 
 def int8_swiglu(x, gate, up, *, x_scales=None, out_dtype=None):
-    """``SiLU(x @ gate.T) * (x @ up.T)`` on 8-bit codes in one product; arguments as ``int8_linear``."""
+    """``SiLU(x @ gate.T) * (x @ up.T)`` on 8-bit codes in one product, in 64 bits up to the one rounding to fp32 (and
+    then to the output type); arguments as ``int8_linear``."""
     if not isinstance(gate, Int8Weight) or not isinstance(up, Int8Weight):
         raise TypeError("gate and up must be Int8Weight")
     if gate.shape != up.shape:

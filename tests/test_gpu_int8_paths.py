@@ -3,14 +3,16 @@
 Sizes are chosen so that the tiles of many tokens are what runs, and ``tiled`` asserts it: codes need a workspace only there.
 (A pair is taken by the few-token kernel up to 256 blocks of 16 channels x 32 tokens.)
 """
+import numpy as np
 import pytest
 import torch
 
+from oracle import int8_np as Q
 from mylocal_llm_amd import _lib
 from mylocal_llm_amd.int8_linear import Int8Weight, int8_linear, int8_quantize, int8_swiglu
 from mylocal_llm_amd.quantized_linear import _TORCH_DTYPE_ID
 from gpu_util import announce
-from test_gpu_int8 import DTYPES, matrix, rows
+from test_gpu_int8 import DTYPES, U, as_np, close, host, matrix, rows
 
 pytestmark = pytest.mark.gpu
 INT8 = 3
@@ -59,7 +61,7 @@ def test_a_token_alone_and_in_a_prompt_gets_the_same_bits(cuda, t, n, k, dtype):
     tiled(t, n, k)
     g, u = pair_of(n, k, t + k)
     codes, scales = int8_quantize(rows(t, k, t))
-    for name, call in both(Int8Weight(*g), Int8Weight(*u), dtype)[:1]:
+    for name, call in both(Int8Weight(*g), Int8Weight(*u), dtype):
         whole = call(codes, scales)
         for lo, hi in ((0, 1), (1, 17), (t - 16, t), (t // 2, t // 2 + 5)):
             part = call(codes[lo:hi].contiguous(), scales[lo:hi].contiguous())
@@ -80,15 +82,58 @@ def test_a_values_bits_do_not_depend_on_where_it_lies(cuda, t, n, k, dtype):
     for m in (n - 1, n - 14, n - 100, n // 2 + 602):
         tiled(t, m, k)
         parts = [Int8Weight(w[0][:m].contiguous(), w[1][:m].contiguous()) for w in (g, u)]
-        for (name, call), want in zip(both(*parts, dtype)[:1], whole):
+        for (name, call), want in zip(both(*parts, dtype), whole):
             got = call(codes, scales)
             assert torch.equal(got, want[:, :m]), (name, m, int((got != want[:, :m]).sum()))
     base = torch.full((t * n + 2,), 3.0, dtype=dtype, device=cuda)
     odt = _TORCH_DTYPE_ID[dtype]
-    for pair, want in enumerate(whole[:1]):
+    for pair, want in enumerate(whole):
         head = [gate.tiles.data_ptr(), gate.scales.data_ptr()] + ([up.tiles.data_ptr(), up.scales.data_ptr()] if pair else [])
         entry = lib.qmoe_int8_swiglu if pair else lib.qmoe_int8_linear
         base.fill_(3.0)
         assert entry(*head, n, k, codes.data_ptr(), INT8, scales.data_ptr(), t, base[1:].data_ptr(), odt, work.data_ptr(), work.numel(), stream) == 0
         torch.cuda.synchronize()
         assert torch.equal(base[1:-1].reshape(t, n), want) and base[0] == 3 and base[-1] == 3
+
+
+@pytest.mark.parametrize("t", [1, 16, 600])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_swiglu_far_below_zero(cuda, t, dtype):
+    """g from -70 to -110, where exp(-g) is beyond fp32 from -88.7 on; u is large, so that silu(g) u is a normal number.
+
+    g and u are sums times scales in 64 bits, h is rounded to fp32 and then to its type: 1.01 * 2^-24 in front of that."""
+    n, k = 2048, 64
+    announce("int8 swiglu far below zero", t, dtype)
+    x = torch.full((t, k), 127, dtype=torch.int8, device=cuda)
+    gate = torch.zeros((n, k), dtype=torch.int8, device=cuda)
+    gate[:, 0] = -127
+    scale = torch.linspace(70, 110, n, device=cuda) / 127 ** 2
+    up = torch.full((n, k), 100, dtype=torch.int8, device=cuda)
+    wide = torch.full((n,), 1e4, device=cuda)
+    one = torch.ones(t, device=cuda)
+    want = Q.swish(Q.product(x.cpu().numpy(), np.ones(t), gate.cpu().numpy(), as_np(scale)), Q.product(x.cpu().numpy(), np.ones(t), up.cpu().numpy(), as_np(wide)))
+    close(int8_swiglu(x, Int8Weight(gate, scale), Int8Weight(up, wide), x_scales=one, out_dtype=dtype), want, 1.01 * U)
+
+
+@pytest.mark.parametrize("t,n,k", [(1, 1601, 512), (16, 2048, 300), (140, 1100, 200), (600, 3584, 256), (4096, 4096, 64)])
+@pytest.mark.parametrize("reach", [0.05, 3.0, 30.0])
+def test_swiglu_is_the_exact_value_rounded(cuda, t, n, k, reach):
+    """From |g| far below one, where 1 + exp(-g) is near two, to hundreds; 2^-46 and the oracle's own error are in the 0.01."""
+    announce("int8 swiglu, 64 bits", t, n, k, reach)
+    g, u = pair_of(n, k, t + n)
+    g[1].mul_(reach)
+    x = rows(t, k, t)
+    q, s = Q.quantize(as_np(x))
+    close(int8_swiglu(x, Int8Weight(*g), Int8Weight(*u)), Q.swish(Q.product(q, s, *host(g)), Q.product(q, s, *host(u))), 1.01 * U)
+
+
+def test_swiglu_of_infinite_scales(cuda):
+    """silu(inf) u is inf u, silu(-inf) is NaN (inf / inf), and so is a sum of 0 times an infinite scale, on both kernels."""
+    n, k = 1100, 64
+    for t in (3, 140):
+        codes = torch.zeros((n, k), dtype=torch.int8, device=cuda)
+        codes[::3, 0], codes[1::3, 0] = 1, -1
+        x, one = torch.ones((t, k), dtype=torch.int8, device=cuda), torch.ones(t, device=cuda)
+        gate, up = Int8Weight(codes, torch.full((n,), float("inf"), device=cuda)), Int8Weight(torch.ones_like(codes), torch.ones(n, device=cuda))
+        got = int8_swiglu(x, gate, up, x_scales=one)
+        assert torch.isposinf(got[:, ::3]).all() and torch.isnan(got[:, 1::3]).all() and torch.isnan(got[:, 2::3]).all()
