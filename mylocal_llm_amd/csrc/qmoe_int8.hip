@@ -91,7 +91,7 @@ template <int DT> static int quantize_as(const void* x, int64_t rows, int k, uin
         return quantize_as<DT>((const char*)x + MOST * k * (int64_t)sizeof(typename Elem<DT>::T), rows - MOST, k, codes + MOST * ld, ld, width, scales + MOST, s);
     }
     const dim3 grid((unsigned)rows);
-    const int eights = (width + 7) / 8;
+    const int64_t eights = ((int64_t)width + 7) / 8;      // (width + 7 of the longest rows passes 32 bits)
     const bool vec = k % 8 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)codes % 8 == 0 && ld % 8 == 0;
     if (eights > (vec ? 8192 : 4096)) {
         hipLaunchKernelGGL(int8_quantize_long_kernel<DT>, grid, dim3(1024), 0, s, x, (int64_t)k, codes, ld, (int64_t)width, scales);
@@ -100,7 +100,7 @@ template <int DT> static int quantize_as(const void* x, int64_t rows, int k, uin
     // Few rows are a chain of latencies: as many threads as there are pieces (one row of 4096 bf16 2.4 us, with two pieces a
     // thread 2.7).  Many rows: more in flight with two (4096 x 4096 bf16 15.1 -> 12.9 us; rows of 512 values 4.5 -> 4.8).
     const int nx = eights > 4096 ? 8 : eights > 2048 ? 4 : eights > 1024 || (rows >= 1024 && eights >= 128) ? 2 : 1;
-    const dim3 block(((eights + nx - 1) / nx + 63) / 64 * 64);
+    const dim3 block((unsigned)(((eights + nx - 1) / nx + 63) / 64 * 64));
 #define QMOE_QUANTIZE(NX, VEC) hipLaunchKernelGGL((int8_quantize_kernel<DT, NX, VEC>), grid, block, 0, s, x, k, codes, ld, width, scales)
     if (nx == 1) { if (vec) QMOE_QUANTIZE(1, true); else QMOE_QUANTIZE(1, false); }
     else if (nx == 2) { if (vec) QMOE_QUANTIZE(2, true); else QMOE_QUANTIZE(2, false); }

@@ -137,3 +137,20 @@ def test_swiglu_of_infinite_scales(cuda):
         gate, up = Int8Weight(codes, torch.full((n,), float("inf"), device=cuda)), Int8Weight(torch.ones_like(codes), torch.ones(n, device=cuda))
         got = int8_swiglu(x, gate, up, x_scales=one)
         assert torch.isposinf(got[:, ::3]).all() and torch.isnan(got[:, 1::3]).all() and torch.isnan(got[:, 2::3]).all()
+
+
+def test_the_longest_row(cuda):
+    """2^31 - 1 columns, where the number of pieces of eight must not be counted in 32 bits."""
+    k = 2 ** 31 - 1
+    announce("int8 longest row")
+    x = torch.zeros((1, k), dtype=torch.float16, device=cuda)
+    places, values = [0, 1, 7, 2 ** 20 + 3, 2 ** 30, k - 8, k - 2, k - 1], [1.0, -0.5, 0.25, -1.0, 0.75, 0.125, -0.996, 1.0]
+    x[0, places] = torch.tensor(values, dtype=torch.float16, device=cuda)
+    want, scale = Q.quantize(as_np(x[:, places]))
+    codes, scales = int8_quantize(x)
+    del x
+    np.testing.assert_array_equal(scales.cpu().numpy(), scale)
+    np.testing.assert_array_equal(codes[:, places].cpu().numpy(), want)
+    assert int(torch.count_nonzero(codes[0, :2 ** 30])) + int(torch.count_nonzero(codes[0, 2 ** 30:])) == len(places)
+    del codes
+    torch.cuda.empty_cache()
