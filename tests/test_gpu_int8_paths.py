@@ -154,3 +154,88 @@ def test_the_longest_row(cuda):
     assert int(torch.count_nonzero(codes[0, :2 ** 30])) + int(torch.count_nonzero(codes[0, 2 ** 30:])) == len(places)
     del codes
     torch.cuda.empty_cache()
+
+
+# ---- what the tiles of many tokens do at the edges ------------------------------------------------------
+
+EDGES = [(140, 1100, 200), (141, 1101, 201), (600, 3584, 256), (1100, 4099, 130)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,n,k", EDGES)
+def test_rows_that_are_not_finite_in_a_prompt(cuda, t, n, k, dtype):
+    announce("int8 prompt with NaN", t, n, k, dtype)
+    tiled(t, n, k)
+    g, u = pair_of(n, k, n + k)
+    gate, up = Int8Weight(*g), Int8Weight(*u)
+    x = rows(t, k, 5, dtype)
+    clean = int8_linear(x, gate), int8_swiglu(x, gate, up)
+    bad = {0: float("nan"), t // 2: float("inf"), t - 1: -float("inf")}
+    for row, value in bad.items():
+        x[row, row % k] = value
+    keep = [i for i in range(t) if i not in bad]
+    for got, want in zip((int8_linear(x, gate), int8_swiglu(x, gate, up)), clean):
+        assert torch.isnan(got[list(bad)]).all() and torch.equal(got[keep], want[keep])
+
+
+def test_extreme_codes_fill_the_int32_sum_of_a_prompt(cuda):
+    t, n, k = 140, 1100, 131071
+    announce("int8 prompt, extreme codes")
+    tiled(t, n, k)
+    codes = torch.full((n, k), -128, dtype=torch.int8, device=cuda)
+    codes[1::2] = 127
+    weight = Int8Weight(codes, torch.ones(n, device=cuda))
+    del codes
+    x = torch.full((t, k), -128, dtype=torch.int8, device=cuda)
+    got = int8_linear(x, weight, x_scales=torch.ones(t, device=cuda))
+    assert got[:, ::2].eq(128.0 * 128 * k).all()
+    assert got[:, 1::2].double().sub(-127.0 * 128 * k).abs().le(127.0 * 128 * k * U).all()
+    x[:, -1] = 127                            # the last column is multiplied, the padding behind it is not
+    got = int8_linear(x, weight, x_scales=torch.ones(t, device=cuda))
+    want = 128.0 * 128 * (k - 1) - 128.0 * 127
+    assert got[:, ::2].double().sub(want).abs().le(want * U).all()
+
+
+def test_prompts_on_two_streams_do_not_meet(cuda):
+    gate, up = (Int8Weight(*m) for m in pair_of(1100, 256, 3))
+    xs = [rows(t, 256, t, dtype) for t, dtype in ((140, torch.float32), (300, torch.bfloat16), (700, torch.float16))]
+    for x in xs:
+        tiled(x.shape[0], 1100, 256)
+    want = [(int8_linear(x, gate), int8_swiglu(x, gate, up)) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = []
+    for _ in range(5):
+        for s, x in zip(streams, xs):
+            with torch.cuda.stream(s):
+                got.append((int8_linear(x, gate), int8_swiglu(x, gate, up)))
+    torch.cuda.synchronize()
+    for i, (a, b) in enumerate(got):
+        assert torch.equal(a, want[i % 3][0]) and torch.equal(b, want[i % 3][1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_prompts_replay_from_two_graphs(cuda, dtype):
+    """Rows quantised on the way, so each graph keeps a workspace of its own."""
+    announce("int8 prompt graphs", dtype)
+    t, n, k = 300, 1100, 256
+    tiled(t, n, k)
+    gate, up = (Int8Weight(*m) for m in pair_of(n, k, 3))
+    x = rows(t, k, 1, dtype)
+    step = lambda: (int8_linear(x, gate), int8_swiglu(x, gate, up))
+    step()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step())
+        graphs.append(graph)
+    for seed in range(4):
+        x.copy_(rows(t, k, seed + 2, dtype))
+        eager = step()
+        torch.cuda.synchronize()
+        for graph, out in zip(graphs, outs):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out[0], eager[0]) and torch.equal(out[1], eager[1])
