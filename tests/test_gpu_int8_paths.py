@@ -3,16 +3,19 @@
 Sizes are chosen so that the tiles of many tokens are what runs, and ``tiled`` asserts it: codes need a workspace only there.
 (A pair is taken by the few-token kernel up to 256 blocks of 16 channels x 32 tokens.)
 """
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
 from oracle import int8_np as Q
-from mylocal_llm_amd import _lib
+from mylocal_llm_amd import _lib, synthetic
 from mylocal_llm_amd.int8_linear import Int8Weight, int8_linear, int8_quantize, int8_swiglu
+from mylocal_llm_amd.int8_moe import Int8ExpertBank, int8_moe_step
 from mylocal_llm_amd.quantized_linear import _TORCH_DTYPE_ID
 from gpu_util import announce
-from test_gpu_int8 import DTYPES, U, as_np, close, host, matrix, rows
+from test_gpu_int8 import DTYPES, U, as_np, close, host, layer, matrix, rows
 
 pytestmark = pytest.mark.gpu
 INT8 = 3
@@ -239,3 +242,100 @@ def test_prompts_replay_from_two_graphs(cuda, dtype):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out[0], eager[0]) and torch.equal(out[1], eager[1])
+
+
+# ---- guards around every output and workspace of the C entries -----------------------------------------
+
+GUARD = 512
+
+
+class Guarded:
+    """A buffer of exactly `nbytes` between two guards, at a 256-byte aligned address."""
+
+    def __init__(self, nbytes, fill=93):
+        self.nbytes, self.fill = nbytes, fill
+        self.bytes = torch.full((nbytes + 2 * GUARD,), fill, dtype=torch.uint8, device="cuda")
+
+    @property
+    def at(self):
+        return self.bytes.data_ptr() + GUARD
+
+    def as_(self, dtype, *shape):
+        return self.bytes[GUARD:GUARD + self.nbytes].view(dtype).reshape(shape)
+
+    def whole(self):
+        return bool(self.bytes[:GUARD].eq(self.fill).all()) and bool(self.bytes[GUARD + self.nbytes:].eq(self.fill).all())
+
+
+@pytest.mark.parametrize("t,n,k", [(1, 70, 200), (5, 71, 200), (16, 70, 129), (19, 70, 200)] + EDGES[:2])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("given", [False, True])
+def test_products_write_their_output_and_workspace_only(cuda, t, n, k, dtype, given):
+    announce("int8 guards", t, n, k, dtype, given)
+    lib, stream = _lib.load(), torch.cuda.current_stream().cuda_stream
+    gate, up = (Int8Weight(*m) for m in pair_of(n, k, 2))
+    x = rows(t, k, 3, dtype)
+    codes, scales = int8_quantize(x)
+    odt = _TORCH_DTYPE_ID[dtype]
+    xdt, xat, sat = (INT8, codes.data_ptr(), scales.data_ptr()) if given else (odt, x.data_ptr(), None)
+    need = lib.qmoe_int8_workspace_bytes(n, k, t, xdt)
+    for pair, want in enumerate((int8_linear(x, gate), int8_swiglu(x, gate, up))):
+        work, out = Guarded(need), Guarded(t * n * x.element_size())
+        head = [gate.tiles.data_ptr(), gate.scales.data_ptr()] + ([up.tiles.data_ptr(), up.scales.data_ptr()] if pair else [])
+        entry = lib.qmoe_int8_swiglu if pair else lib.qmoe_int8_linear
+        assert entry(*head, n, k, xat, xdt, sat, t, out.at, odt, work.at if need else None, need, stream) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(out.as_(dtype, t, n), want) and out.whole() and work.whole()
+
+
+@pytest.mark.parametrize("t", [1, 4, 5, 16, 17, 60])
+@pytest.mark.parametrize("e,k,d,f,fs", [(12, 4, 160, 96, 64), (7, 3, 65, 33, 17), (40, 2, 128, 64, 0)])
+@pytest.mark.parametrize("routed", [False, True])
+def test_step_writes_its_outputs_and_workspace_only(cuda, t, e, k, d, f, fs, routed):
+    announce("int8 step guards", t, e, k, d, f, fs, routed)
+    lib, stream = _lib.load(), torch.cuda.current_stream().cuda_stream
+    parts, shared, vec = layer(e, d, f, fs, 3)
+    bank, dshared = Int8ExpertBank(*parts), tuple(Int8Weight(*m) for m in shared) if shared else None
+    x, residual, logits = rows(t, d, 1, torch.bfloat16), rows(t, d, 2), torch.from_numpy(synthetic.router_logits(t, e, 3)).cuda()
+    want, w, ids = int8_moe_step(x, bank, k, logits=logits, shared=dshared, shared_gate=vec, residual=residual, return_routing=True)
+    need = lib.qmoe_int8_moe_workspace_bytes(t, k, e, d, f, fs)
+    work, out, out_w, out_i, status = Guarded(need), Guarded(t * d * 2), Guarded(t * k * 4), Guarded(t * k * 8), Guarded(4, 0)
+    a = _lib.Int8MoeArgs()
+    a.hidden, a.hidden_dtype, a.tokens, a.top_k = x.data_ptr(), _TORCH_DTYPE_ID[x.dtype], t, k
+    a.floor_value, a.renormalize = 2.0 ** -14, 1
+    if routed:
+        a.in_weights, a.in_ids = w.data_ptr(), ids.data_ptr()
+    else:
+        a.logits = logits.data_ptr()
+    a.gate, a.up, a.down = bank.gate_tiles.data_ptr(), bank.up_tiles.data_ptr(), bank.down_tiles.data_ptr()
+    a.gate_scales, a.up_scales, a.down_scales = bank.gate_scales.data_ptr(), bank.up_scales.data_ptr(), bank.down_scales.data_ptr()
+    a.n_experts, a.d_model, a.d_ff, a.d_ff_shared = e, d, f, fs
+    if fs:
+        a.shared_gate_w, a.shared_up_w, a.shared_down_w = (m.tiles.data_ptr() for m in dshared)
+        a.shared_gate_scales, a.shared_up_scales, a.shared_down_scales = (m.scales.data_ptr() for m in dshared)
+        a.shared_gate = vec.data_ptr()
+    a.out, a.out_dtype, a.out_weights, a.out_ids = out.at, a.hidden_dtype, out_w.at, out_i.at
+    a.residual, a.status_out = residual.data_ptr(), status.at
+    assert lib.qmoe_int8_moe_forward(ctypes.byref(a), work.at, need, stream) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(out.as_(torch.bfloat16, t, d), want) and torch.equal(out_w.as_(torch.float32, t, k), w) and torch.equal(out_i.as_(torch.int64, t, k), ids)
+    assert not status.bytes.any()
+    assert work.whole() and out.whole() and out_w.whole() and out_i.whole()
+    assert lib.qmoe_int8_moe_forward(ctypes.byref(a), work.at, need - 1, stream) == 4      # the size above is needed whole
+
+
+@pytest.mark.parametrize("big,small", [(16, 1), (16, 4), (16, 5), (17, 16), (17, 4), (40, 16), (130, 1), (130, 17)])
+@pytest.mark.parametrize("fs", [0, 128])
+def test_a_tokens_step_has_the_same_bits_in_every_batch(cuda, big, small, fs):
+    """Codes, sums, hidden activations and the order of additions are the same on every path.  (The shared expert's admission
+    gate is left out: its fp32 dot product is added in another order beyond 16 tokens.)"""
+    announce("int8 step in batches", big, small, fs)
+    e, k, d, f = 24, 4, 256, 192
+    parts, shared, _ = layer(e, d, f, fs, 6)
+    bank, dshared = Int8ExpertBank(*parts), tuple(Int8Weight(*m) for m in shared) if shared else None
+    x, residual, logits = rows(big, d, 2), rows(big, d, 3), torch.from_numpy(synthetic.router_logits(big, e, 3)).cuda()
+    whole = int8_moe_step(x, bank, k, logits=logits, shared=dshared, residual=residual)
+    for lo in (0, big - small):
+        s = slice(lo, lo + small)
+        part = int8_moe_step(x[s].contiguous(), bank, k, logits=logits[s].contiguous(), shared=dshared, residual=residual[s].contiguous())
+        assert torch.equal(whole[s], part)
