@@ -195,7 +195,6 @@ struct Int8Product {
     const int *chunk_expert, *chunk_start, *chunk_count, *n_chunks;
     int64_t w_step;                   // bytes of one expert's matrix
     const int* row_of;                // sorted position -> row of q (NULL: the position itself)
-    int hidden;                       // pair: store the expert's hidden activation (int8_hidden)
 };
 
 }  // namespace qmoe

@@ -365,7 +365,7 @@ static int int8_moe_impl(const qmoe_int8_moe_args& m, char* ws, const Int8MoeLay
     p.w = (const uint8_t*)m.gate; p.w2 = (const uint8_t*)m.up; p.c = m.gate_scales; p.c2 = m.up_scales;
     p.n = f; p.kp = (int)int8_cols64(d); p.w_step = int8_matrix_bytes(f, d);
     p.q = (const uint8_t*)(ws + L.q); p.ld = dp; p.s = (const float*)(ws + L.s);
-    p.y = ws + L.h; p.ydt = QMOE_DT_F32; p.ldy = f; p.hidden = 1; p.tokens = t;
+    p.y = ws + L.h; p.ydt = QMOE_DT_F32; p.ldy = f; p.tokens = t;
     p.chunk_expert = (const int*)(ws + L.chunk_expert); p.chunk_start = (const int*)(ws + L.chunk_start);
     p.chunk_count = (const int*)(ws + L.chunk_count); p.n_chunks = (const int*)(ws + L.n_chunks);
     p.row_of = (const int*)(ws + L.row_of);
@@ -373,7 +373,7 @@ static int int8_moe_impl(const qmoe_int8_moe_args& m, char* ws, const Int8MoeLay
     Int8Product g{};
     if (fs) {
         g.w = (const uint8_t*)m.shared_gate_w; g.w2 = (const uint8_t*)m.shared_up_w; g.c = m.shared_gate_scales; g.c2 = m.shared_up_scales;
-        g.n = fs; g.kp = p.kp; g.q = p.q; g.ld = dp; g.s = p.s; g.tokens = t; g.y = ws + L.sh; g.ydt = QMOE_DT_F32; g.ldy = fs; g.hidden = 1;
+        g.n = fs; g.kp = p.kp; g.q = p.q; g.ld = dp; g.s = p.s; g.tokens = t; g.y = ws + L.sh; g.ydt = QMOE_DT_F32; g.ldy = fs;
     }
     if ((rc = int8_plan_launch(p, true, rows, max_chunks, fs ? &g : nullptr, s))) return rc;
     const Int8Rows routed{(const float*)(ws + L.h), f, fp, (uint8_t*)(ws + L.hq), (float*)(ws + L.hs)};
@@ -382,7 +382,7 @@ static int int8_moe_impl(const qmoe_int8_moe_args& m, char* ws, const Int8MoeLay
     if ((rc = check_launch("int8 expert step (codes)"))) return rc;
     Int8Product q = p;
     q.w = (const uint8_t*)m.down; q.c = m.down_scales; q.n = d; q.kp = (int)int8_cols64(f); q.w_step = int8_matrix_bytes(d, f);
-    q.q = (const uint8_t*)(ws + L.hq); q.ld = fp; q.s = (const float*)(ws + L.hs); q.y = ws + L.terms; q.ldy = d; q.hidden = 0;
+    q.q = (const uint8_t*)(ws + L.hq); q.ld = fp; q.s = (const float*)(ws + L.hs); q.y = ws + L.terms; q.ldy = d;
     q.row_of = nullptr;
     Int8Product o{};
     if (fs) {
