@@ -326,16 +326,18 @@ def test_step_writes_its_outputs_and_workspace_only(cuda, t, e, k, d, f, fs, rou
 
 @pytest.mark.parametrize("big,small", [(16, 1), (16, 4), (16, 5), (17, 16), (17, 4), (40, 16), (130, 1), (130, 17)])
 @pytest.mark.parametrize("fs", [0, 128])
-def test_a_tokens_step_has_the_same_bits_in_every_batch(cuda, big, small, fs):
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_tokens_step_has_the_same_bits_in_every_batch(cuda, big, small, fs, dtype):
     """Codes, sums, hidden activations and the order of additions are the same on every path.  (The shared expert's admission
     gate is left out: its fp32 dot product is added in another order beyond 16 tokens.)"""
-    announce("int8 step in batches", big, small, fs)
+    announce("int8 step in batches", big, small, fs, dtype)
     e, k, d, f = 24, 4, 256, 192
     parts, shared, _ = layer(e, d, f, fs, 6)
     bank, dshared = Int8ExpertBank(*parts), tuple(Int8Weight(*m) for m in shared) if shared else None
     x, residual, logits = rows(big, d, 2), rows(big, d, 3), torch.from_numpy(synthetic.router_logits(big, e, 3)).cuda()
-    whole = int8_moe_step(x, bank, k, logits=logits, shared=dshared, residual=residual)
+    whole = int8_moe_step(x, bank, k, logits=logits, shared=dshared, residual=residual, out_dtype=dtype)
     for lo in (0, big - small):
         s = slice(lo, lo + small)
-        part = int8_moe_step(x[s].contiguous(), bank, k, logits=logits[s].contiguous(), shared=dshared, residual=residual[s].contiguous())
+        part = int8_moe_step(x[s].contiguous(), bank, k, logits=logits[s].contiguous(), shared=dshared, residual=residual[s].contiguous(),
+                             out_dtype=dtype)
         assert torch.equal(whole[s], part)
