@@ -158,6 +158,23 @@ __device__ __forceinline__ float int8_hidden(double g, double u) {
     return to_fp32(g * i * u);
 }
 
+// sigmoid(x . w) of a token's row by one wave: what admits the shared expert.  In fp32, and in one order of additions whichever
+// kernel asks, so that a token's step has the same bits in every batch.
+template <int XDT> __device__ __forceinline__ float int8_admission(const void* x, size_t row, bool fast, const float* w, bool w_fast, int d) {
+    float sum = 0.0f;
+#pragma unroll 4
+    for (int i = (int)(threadIdx.x & 63) * 8; i < d; i += 512) {
+        float a[8], b[8], t[4];
+        int8_load8<XDT>(x, row + i, d - i, fast, a);
+        int8_load8<QMOE_DT_F32>(w, i, d - i, w_fast, b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t[j] = __builtin_fmaf(a[2 * j + 1], b[2 * j + 1], __fmul_rn(a[2 * j], b[2 * j]));
+        sum += (t[0] + t[1]) + (t[2] + t[3]);
+    }
+    sum = wave_sum(sum);
+    return sum >= 0.0f ? 1.0f / (1.0f + expf(-sum)) : expf(sum) / (1.0f + expf(sum));
+}
+
 // LDS operations of this workgroup's waves before and after; requests for memory stay in flight.
 __device__ __forceinline__ void meet_lds() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");

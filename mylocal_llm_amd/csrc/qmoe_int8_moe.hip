@@ -234,7 +234,7 @@ __global__ __launch_bounds__(256) void int8_combine_kernel(const float* __restri
                                                            const void* __restrict__ x, const float* __restrict__ residual,
                                                            void* __restrict__ out, int odt) {
     __shared__ int pos[32];
-    __shared__ float weight[32], partial[4];
+    __shared__ float weight[32], admitted;
     __shared__ int kept;
     const int64_t t = blockIdx.x;
     const int tid = threadIdx.x;
@@ -250,24 +250,15 @@ __global__ __launch_bounds__(256) void int8_combine_kernel(const float* __restri
         if (p >= 0) { pos[rank] = p; weight[rank] = weights[t * k + tid]; }
         if (tid == 0) kept = n;
     }
-    float admit = 1.0f;
-    const bool wide = d % 4 == 0 && ((uintptr_t)x | (uintptr_t)shared_gate | (uintptr_t)residual | (uintptr_t)out) % 16 == 0;
-    if (shared_out && shared_gate) {
-        float a = 0.0f;
-        if (wide)
-            for (int i = 4 * tid; i < d; i += 1024) {
-                const float4 h = Elem<XDT>::load4(x, (size_t)t * d + i), g = ldg<float4>(shared_gate + i);
-                a += (h.x * g.x + h.y * g.y) + (h.z * g.z + h.w * g.w);
-            }
-        else
-            for (int i = tid; i < d; i += 256) a += Elem<XDT>::load(x, (size_t)t * d + i) * shared_gate[i];
-        a = wave_sum(a);
-        if ((tid & 63) == 0) partial[tid >> 6] = a;
-        __syncthreads();
-        a = (partial[0] + partial[1]) + (partial[2] + partial[3]);
-        admit = a >= 0.0f ? 1.0f / (1.0f + expf(-a)) : expf(a) / (1.0f + expf(a));
+    else if (tid < 128) {        // the second wave: the shared expert's admission
+        const bool eights = d % 8 == 0;
+        const float a = shared_out && shared_gate ? int8_admission<XDT>(x, (size_t)t * d, eights && (uintptr_t)x % 16 == 0, shared_gate,
+                                                                          eights && (uintptr_t)shared_gate % 16 == 0, d) : 1.0f;
+        if (tid == 64) admitted = a;
     }
     __syncthreads();
+    const float admit = admitted;
+    const bool wide = d % 4 == 0 && ((uintptr_t)x | (uintptr_t)shared_gate | (uintptr_t)residual | (uintptr_t)out) % 16 == 0;
     if (wide) {
         // four columns a thread; eight terms' requests leave together, the adds follow in order
         for (int i = 4 * tid; i < d; i += 1024) {

@@ -365,17 +365,8 @@ __global__ __launch_bounds__(64 * WAVES) void int8_front_kernel(const Front8Args
     }
     if (a.admit_w && wave == WAVES - 1) {
         for (int t = (G + G - 2 - (int)blockIdx.x) % G; t < tokens; t += G) {
-            float sum = 0.0f;
-#pragma unroll 4
-            for (int i = lane * 8; i < a.d; i += 512) {
-                float x[8], w[8];
-                int8_load8<XDT>(a.x, (size_t)t * a.d + i, a.d - i, a.fast, x);
-                int8_load8<QMOE_DT_F32>(a.admit_w, i, a.d - i, a.fast && a.admit_fast, w);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) sum += x[j] * w[j];
-            }
-            sum = wave_sum(sum);
-            if (lane == 0) a.o.admit[t] = sum >= 0.0f ? 1.0f / (1.0f + expf(-sum)) : expf(sum) / (1.0f + expf(sum));
+            const float admit = int8_admission<XDT>(a.x, (size_t)t * a.d, a.fast, a.admit_w, a.fast && a.admit_fast, a.d);
+            if (lane == 0) a.o.admit[t] = admit;
         }
     }
 }

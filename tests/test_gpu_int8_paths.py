@@ -328,8 +328,7 @@ def test_step_writes_its_outputs_and_workspace_only(cuda, t, e, k, d, f, fs, rou
 @pytest.mark.parametrize("fs", [0, 128])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_a_tokens_step_has_the_same_bits_in_every_batch(cuda, big, small, fs, dtype):
-    """Codes, sums, hidden activations and the order of additions are the same on every path.  (The shared expert's admission
-    gate is left out: its fp32 dot product is added in another order beyond 16 tokens.)"""
+    """Codes, sums, hidden activations and the order of additions are the same on every path."""
     announce("int8 step in batches", big, small, fs, dtype)
     e, k, d, f = 24, 4, 256, 192
     parts, shared, _ = layer(e, d, f, fs, 6)
@@ -341,3 +340,19 @@ def test_a_tokens_step_has_the_same_bits_in_every_batch(cuda, big, small, fs, dt
         part = int8_moe_step(x[s].contiguous(), bank, k, logits=logits[s].contiguous(), shared=dshared, residual=residual[s].contiguous(),
                              out_dtype=dtype)
         assert torch.equal(whole[s], part)
+
+
+@pytest.mark.parametrize("big,small,d", [(17, 16, 256), (40, 4, 300), (130, 1, 1031), (60, 5, 2048)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_the_shared_experts_admission_has_the_same_bits_in_every_batch(cuda, big, small, d, dtype):
+    """The gate's dot product of fp32 is added in one order, whether a front kernel or a prompt's combine forms it."""
+    announce("int8 admission in batches", big, small, d, dtype)
+    e, k, f, fs = 12, 2, 64, 96
+    parts, shared, vec = layer(e, d, f, fs, 6)
+    bank, dshared = Int8ExpertBank(*parts), tuple(Int8Weight(*m) for m in shared)
+    x, logits = rows(big, d, 2, dtype), torch.from_numpy(synthetic.router_logits(big, e, 3)).cuda()
+    whole = int8_moe_step(x, bank, k, logits=logits, shared=dshared, shared_gate=vec, out_dtype=torch.float32)
+    for lo in range(0, big - small + 1, small):
+        s = slice(lo, lo + small)
+        part = int8_moe_step(x[s].contiguous(), bank, k, logits=logits[s].contiguous(), shared=dshared, shared_gate=vec, out_dtype=torch.float32)
+        assert torch.equal(whole[s], part), (lo, int((whole[s] != part).sum()))
