@@ -332,7 +332,8 @@ int qmoe_int8_swiglu(const void* gate, const float* gate_scales, const void* up,
 /* One MoE step on such weights.  Host struct; fields as in qmoe_moe_args, matrices as tiles: gate / up
  * n_experts x [d_ff, d_model], down n_experts x [d_model, d_ff], each with fp32 channel scales
  * [n_experts, rows]; the shared expert (all NULL and d_ff_shared = 0: none) likewise.  Every expert's
- * hidden activation is rounded to fp32 and quantised per (token, expert) before its down projection. */
+ * hidden activation is rounded to fp32 and quantised per (token, expert) before its down projection.
+ * A token's output has the same bits in every batch. */
 typedef struct qmoe_int8_moe_args {
     const void* hidden;
     int hidden_dtype;

@@ -5,8 +5,8 @@ namespace qmoe {
 
 // ---- rows -> codes + scales ------------------------------------------------------------------------------
 // One workgroup a row, NX pieces of eight values a thread in registers between the search for the largest and the
-// codes: a row is read once.  Bound by the memory for many rows (cold, 4096 x 4096: fp32 15.1 us, 5.6 TB/s of
-// reads and writes; bf16 13.0 us, 3.9 TB/s), by one round trip and one meeting for a few (1 x 4096 2.0 - 2.4 us, launch included).
+// codes: a row is read once.  Bound by the memory for many rows (4096 x 4096, a dozen inputs in turn: fp32 15.1 us, 5.6 TB/s of
+// reads and writes; bf16 11.2 us, 4.5 TB/s, or 13.2 where half the waves hold a value next to a half), by one round trip and one meeting for a few (1 x 4096 2.0 - 2.4 us, launch included).
 //   vec   a row starts 16-byte aligned and ends on a multiple of eight values: 16-byte loads, 8-byte stores
 //   else  neighbouring threads take neighbouring values: whole lines still, 2 or 4 bytes a thread
 template <int DT, int NX, bool VEC>

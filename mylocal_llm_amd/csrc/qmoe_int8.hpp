@@ -60,8 +60,9 @@ __device__ __forceinline__ int int8_code_slow(float x, double inv) {
 }
 // N values' codes as bytes.  u = x * inv + 1.5 * 2^23 in one fma holds the nearest whole number in its low bits; x * inv is
 // within 127 * 2^-24 < 2^-17 of x / s, so wherever it is no closer than 2^-16 to a half that number is the code.  The rest,
-// one wave of 512 values in thirty of fp32 rows and more of 16-bit ones (half the largest is 63.5 s), is decided in 64 bits.
-// (The sign of x - (n + 1/2) s, one fp32 fma, decides as well and was no faster: 4096 x 4096 bf16 12.9 / 13.0 us.)
+// one wave of 512 values in 64 of fp32 rows, is decided in 64 bits; of 16-bit rows about half the waves if they are N(0, 1): half
+// the largest is 63.5 s, and there are few values to fall on.  (4096 x 4096 bf16: 13.2 us so, 11.2 where a few loud channels hold
+// the largest.  The sign of x - (n + 1/2) s, one fp32 fma, decides as well and was no faster: 12.9 / 13.0 us.)
 template <int N> __device__ __forceinline__ void int8_codes(const float* v, const RowScale& r, uint32_t* out) {
     const float magic = 12582912.0f;
     uint32_t u[N];

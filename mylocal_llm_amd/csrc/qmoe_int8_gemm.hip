@@ -165,8 +165,8 @@ __global__ __launch_bounds__(64 * WN * WT) __attribute__((amdgpu_waves_per_eu(2)
         if (c0 + h < chunks) turn(c0 + h, h);
     // D[j] of a lane: channel 4 g + j of the tile, token col.  One formula for every value, whatever its type, its place and its
     // neighbours: scaled in 64 bits and rounded to fp32, then to the type, as for a few tokens.  (Scaling 16-bit results in fp32 saves
-    // nothing: from codes, 4096 x 14336 x 4096 bf16 212 us so, 209 in 64 bits.)  The type is decided once, not for each value: the unrolled code runs once a
-    // workgroup, and its size is its time.
+    // nothing: from codes, 4096 x 14336 x 4096 bf16 212 us so, 209 in 64 bits.)  The type is decided once, not for each value: the
+    // unrolled code runs once a workgroup, and its size is its time.
     auto value = [&](int i, int t, int j, float s, double c, double c2) -> float {
         const double y = (double)acc[i * NP][t][j] * ((double)s * c);
         if (!PAIR) return to_fp32(y);
@@ -250,7 +250,7 @@ int int8_plan_rows(int64_t assignments, int n_experts) {
     const int64_t average = assignments / n_experts;
     return average < 28 ? 32 : average <= 72 ? 64 : 128;
 }
-// side: NULL, or a dense product of the same kind (pair with the hidden activation, or plain) that rides in front.
+// side: NULL, or a dense product of the same kind (pair or plain) that rides in front.
 int int8_plan_launch(const Int8Product& a, bool pair, int rows, int max_chunks, const Int8Product* side, hipStream_t s) {
     if (pair) {
         if (rows == 32) return gemm8_as<true, true, 4, 1, 1, 2, 256, 8, 2>(a, max_chunks, s, side);
@@ -269,8 +269,9 @@ int int8_plan_launch(const Int8Product& a, bool pair, int rows, int max_chunks, 
 // 7.7, 128 x 4096 x 4096 - / - / 18 / 13 / 12.4 / 10.0 / 12.2, 64 x 4096 x 14336 - / - / - / - / 35 / 27 / 20.
 // One workgroup a CU loses what the last round leaves empty, and nothing hides its start and its end: the largest tile is
 // taken where the rounds come out nearly even.
-// What bounds it: large sizes the matrix instructions and what feeds them (4096 x 4096 x 14336 2.8 POP/s, of 4.8 that the
-// instruction alone reaches), small ones the way from one chunk to the next, 0.2 - 0.4 us of meeting and latencies.
+// (Measured when the rule was made; the kernels have gained 2 - 10 % since, alike.)
+// What bounds it: large sizes the matrix instructions and what feeds them (4096 x 4096 x 14336 173 - 187 us from run to
+// run, 2.6 - 2.8 POP/s, of 4.8 that the instruction alone reaches), small ones the way from one chunk to the next, 0.2 - 0.4 us of meeting and latencies.
 int int8_gemm_launch(const Int8Product& a, bool pair, hipStream_t s) {
     auto blocks = [&](int channels, int tokens) {
         return (int64_t)((a.n + channels - 1) / channels) * ((a.tokens + tokens - 1) / tokens);

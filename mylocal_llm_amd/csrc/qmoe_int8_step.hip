@@ -1,4 +1,6 @@
-// The expert step for up to 16 tokens: routing + gate/up in front, down + combine behind.
+// The expert step for up to 16 tokens: routing + gate/up in front, down + combine behind.  The back kernel holds the codes of
+// every (token, expert) row in LDS at once, 140 KB of them: int8_step_covers.  That is 16 tokens of 10 x 512 and a shared expert of
+// 2048 (3.5 KB to spare) or of 8 x 768, 11 of 6 x 1408 and 2816, 10 of 8 x 1536, 4 of 2 x 14336; more tokens take the prompt's step.
 //
 //   front   Every workgroup routes the tokens and quantises their rows itself (nothing waits for another workgroup), then
 //           streams its items: 16 channels of the gate and the up matrix of one expert, shared expert's first.
@@ -14,9 +16,9 @@
 // another inside the stream.  Requests run R steps ahead through a ring of registers.
 //
 // Measured at 512 experts, ten a token, 2048 columns, width 512, shared expert of 2048, weights from memory:
-//   1 token    front 13.6 us, back 9.4 us for 44 MB: two launches, each a chain of latencies (launch 2, logits and rows 2,
+//   1 token    front 13.3 us, back 9.3 us for 44 MB: two launches, each a chain of latencies (launch 2, logits and rows 2,
 //              selection 1, first weights 2 us) around 4 - 5 us of streaming
-//   16 tokens  routing 6.0, front 61.6 (300 MB, 4.9 TB/s), codes 4.7, back 34.6 us (150 MB, 4.3 TB/s)
+//   16 tokens  routing 6.1, front 62.3 (300 MB, 4.8 TB/s), codes 4.7, back 34.8 us (150 MB, 4.3 TB/s)
 #include "qmoe_int8_route.hpp"
 
 namespace qmoe {
