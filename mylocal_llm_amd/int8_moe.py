@@ -23,9 +23,27 @@ def _workspace_bytes(*sizes):
     return _lib.load().qmoe_int8_moe_workspace_bytes(*sizes)
 
 
+def _held(name):
+    """A bank's tensor.  Another may take its place if it is what the kernels read there."""
+    slot = "_" + name
+
+    def put(self, tensor):
+        old = getattr(self, slot)
+        if not isinstance(tensor, torch.Tensor) or tensor.dtype != old.dtype or tensor.shape != old.shape or not tensor.is_contiguous():
+            raise ValueError(f"{name} must be contiguous {str(old.dtype)[6:]} {list(old.shape)}")
+        if tensor.device != old.device:
+            raise ValueError("all matrices of a bank must be on the same device")
+        setattr(self, slot, tensor)
+
+    return property(lambda self: getattr(self, slot), put)
+
+
 class Int8ExpertBank:
     """E SwiGLU experts: ``gate`` and ``up`` are (codes int8 [E, F, D], scales fp32 [E, F]) pairs, ``down`` is
     (codes int8 [E, D, F], scales fp32 [E, D]), contiguous on one device."""
+
+    gate_tiles, up_tiles, down_tiles = _held("gate_tiles"), _held("up_tiles"), _held("down_tiles")
+    gate_scales, up_scales, down_scales = _held("gate_scales"), _held("up_scales"), _held("down_scales")
 
     def __init__(self, gate, up, down):
         for name, pair in (("gate", gate), ("up", up), ("down", down)):
@@ -44,17 +62,20 @@ class Int8ExpertBank:
                    (gate[1], up[1], down[1]), e, d, f)
 
     def _hold(self, tiles, scales, e, d, f):
-        self.gate_tiles, self.up_tiles, self.down_tiles = tiles
-        self.gate_scales, self.up_scales, self.down_scales = scales
+        self._gate_tiles, self._up_tiles, self._down_tiles = tiles
+        self._gate_scales, self._up_scales, self._down_scales = scales
+        self._sizes = tuple(t.numel() for t in (*tiles, *scales))
         self.n_experts, self.d_model, self.d_ff = e, d, f
         self.device = tiles[0].device
 
     def fill(self, args):
         """The bank's part of a step's argument struct.  Addresses are read from the tensors at every call: one kept from an
         earlier call would be stale, or free, once a tensor is replaced."""
-        args.gate, args.up, args.down = self.gate_tiles.data_ptr(), self.up_tiles.data_ptr(), self.down_tiles.data_ptr()
-        args.gate_scales, args.up_scales, args.down_scales = (
-            self.gate_scales.data_ptr(), self.up_scales.data_ptr(), self.down_scales.data_ptr())
+        gate, up, down, gs, us, ds = (self._gate_tiles, self._up_tiles, self._down_tiles, self._gate_scales, self._up_scales, self._down_scales)
+        if (gate.numel(), up.numel(), down.numel(), gs.numel(), us.numel(), ds.numel()) != self._sizes:
+            raise ValueError("a tensor of the bank was resized")
+        args.gate, args.up, args.down = gate.data_ptr(), up.data_ptr(), down.data_ptr()
+        args.gate_scales, args.up_scales, args.down_scales = gs.data_ptr(), us.data_ptr(), ds.data_ptr()
         args.n_experts, args.d_model, args.d_ff = self.n_experts, self.d_model, self.d_ff
 
     @classmethod
